@@ -17,13 +17,14 @@ import torch  # noqa: F401  (loads torch's HIP runtime first)
 LIB_PATH = Path(__file__).resolve().parent / "libdiffucore_amd.so"
 
 F16, BF16, F32, I32, NONE = 0, 1, 2, 3, -1
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _DTYPE = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.int32: I32}
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_Z = ctypes.c_size_t
 _SIGS = {
     "dc_last_error": (ctypes.c_char_p, []),
     "dc_abi_version": (_I, []),
@@ -55,6 +56,18 @@ _SIGS = {
                                       ctypes.POINTER(_I64), ctypes.POINTER(_I64), ctypes.POINTER(_I64),
                                       ctypes.POINTER(_I64), ctypes.c_float, _P]),
     "dc_int8_attn_quantize_q": (_I, [_P, _I, _I, _I, _I, _I, ctypes.POINTER(_I64), _P, _P, _P]),
+    "dc_linear16_workspace_bytes": (_Z, [_I, _I64, _I64, _I64]),
+    "dc_linear16": (_I, [_P, _I64, _P, _I64, _P, _I, _P, _I64, _I, _P, _I64, _P, _I64, _I, _I64, _I64, _I64, _P, _Z, _P]),
+    "dc_gated16": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64,
+                        _P, _Z, _P]),
+    "dc_linear16_dx": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _I, _I64, _I64, _I64, _P, _Z, _P]),
+    "dc_linear16_dw": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I, _I64, _I64, _I64, _P, _Z, _P]),
+    "dc_act16_bwd_workspace_bytes": (_Z, [_I64, _I64, _I]),
+    "dc_act16_bwd": (_I, [_P, _I64, _P, _I64, _I, _P, _I64, _P, _I, _I, _I64, _I64, _P, _Z, _P]),
+    "dc_gated16_bwd": (_I, [_P, _I64, _P, _P, _I64, _I, _P, _P, _I64, _P, _P, _I, _I, _I64, _I64, _P, _Z, _P]),
+    "dc_layer_norm": (_I, [_P, _I64, _I, _P, _P, _I, ctypes.c_float, _P, _I64, _P, _I64, _I64, _P]),
+    "dc_layer_norm_bwd_workspace_bytes": (_Z, [_I64, _I64, _I]),
+    "dc_layer_norm_bwd": (_I, [_P, _I64, _P, _I64, _I, _P, _I, _P, _P, _I64, _P, _P, _I64, _I64, _P, _Z, _P]),
     "dc_mfma_probe": (_I, [_I, _I, _I, _I, _P, _P]),
     "dc_mfma_probe_units": (_I, []),
 }

@@ -25,7 +25,7 @@
 //   d4  - within 4 consecutive elements (in registers)
 // Each H4 step is y[j] = S - 2*x[3-j] with S = (x0 + x1) + (x2 + x3), applied
 // along d1, d2, d3, d4 in that order; the result is scaled by 1/16 (exact).
-#include "common.h"
+#include "act.h"
 
 namespace dc {
 
@@ -331,60 +331,16 @@ __global__ void __launch_bounds__(1024) quant_rows_lds_kernel(const void* __rest
 
 // ---------------------------------------------------------------- activation + concatenation
 
-// GELU in float32, then rounded to the 16-bit type DT as the reference rounds
-// it (src/diffucore/models/_int8.py:433-435: 0.5 h (1 + erf(h / sqrt 2)),
-// cast to the activation dtype; the tanh form is torch's
-// gelu(approximate="tanh"), 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))),
-// which FLUX's MLPs use). Both are evaluated in forms without the cancellation
-// the textbook forms have in the negative tail, with the hardware exp2 /
-// reciprocal (this pass is VALU-bound, and the library erf / tanh cost about
-// twice as much):
-//   tanh form: 0.5 x (1 + tanh u) = x / (1 + 2^(-2 u log2 e));
-//   erf form: 1 + erf(x / sqrt 2) = erfc(z) for x < 0, 2 - erfc(z) for x >= 0,
-//   z = |x| / sqrt 2, erfc by the Chebyshev-fitted form of Press et al.,
-//   Numerical Recipes (2nd ed., section 6.2, erfcc): t = 1 / (1 + z / 2),
-//   erfc(z) = t exp(-z^2 - 1.26551223 + t P(t)) with P of degree 9, whose
-//   relative error is below 1.2e-7 for every z >= 0.
-// Both keep a small relative error over the whole line. The reference's
-// cancelling forms do not: below x = -4 or so their float32 1 + erf / 1 + tanh
-// sits on the 2^-24 grid, and below about -5.5 they return -0. There the
-// values here are the accurate ones, so the 16-bit results can differ from the
-// reference's; those elements are below 1e-4 in magnitude (codes 0 unless a
-// whole row lies that far out). Elsewhere the two agree to a few float32 ulp,
-// which the rounding to 16 bits hides except next to a boundary.
-constexpr float LOG2E = 1.4426950408889634f;
-
-// The constants of u, log2 e, the 1 / sqrt 2 of z and the 0.5 are folded into
-// the coefficients: x * x is exact in float32 for a 16-bit x, so both forms
-// round less often than with z and u written out. Largest relative error over
-// all finite 16-bit |x| < 10 with exact exp2 / reciprocal, before -> now: tanh
-// form 1.0e-5 -> 6.3e-6, erf form 7.5e-6 -> 3.3e-6 (both in the far negative
-// tail; 1.7e-6 -> 1.4e-6 and 2.2e-6 -> 9e-7 for |x| < 5).
-__device__ __forceinline__ float gelu_tanh_f32(float x) {
-  // -2 u log2 e = x (A + B x^2), A = -2 log2 e sqrt(2 / pi) and B = 0.044715 A each rounded once
-  constexpr float A = -2.302208198144325f, B = -0.1029432395800235f;
-  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * __builtin_fmaf(x * x, B, A)));
-}
-
-__device__ __forceinline__ float gelu_erf_f32(float x) {
-  // h = erfc(z) / 2 = t 2^(log2 e (-z^2 - 1.26551223 + t P(t)) - 1), z^2 = x^2 / 2
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f * 0.7071067811865476f, fabsf(x), 1.0f));
-  float p = __builtin_fmaf(0.17087277f * LOG2E, t, -0.82215223f * LOG2E);
-  p = __builtin_fmaf(p, t, 1.48851587f * LOG2E);
-  p = __builtin_fmaf(p, t, -1.13520398f * LOG2E);
-  p = __builtin_fmaf(p, t, 0.27886807f * LOG2E);
-  p = __builtin_fmaf(p, t, -0.18628806f * LOG2E);
-  p = __builtin_fmaf(p, t, 0.09678418f * LOG2E);
-  p = __builtin_fmaf(p, t, 0.37409196f * LOG2E);
-  p = __builtin_fmaf(p, t, 1.00002368f * LOG2E);
-  p = __builtin_fmaf(p, t, -1.26551223f * LOG2E - 1.0f);
-  const float h = t * __builtin_amdgcn_exp2f(__builtin_fmaf(x * x, -0.5f * LOG2E, p));
-  // the float's sign, not the 16-bit input's: comparing that would keep the
-  // packed inputs live to the end (fp16: 58 VGPRs, 8 waves per SIMD; 68 and 7)
-  x = materialize(x);
-  return x * (x < 0.0f ? h : 1.0f - h);
-}
-
+// The GELU (act.h) is rounded to the 16-bit type DT as the reference rounds it
+// (src/diffucore/models/_int8.py:433-435: 0.5 h (1 + erf(h / sqrt 2)), cast to
+// the activation dtype; the tanh form is torch's gelu(approximate="tanh"),
+// which FLUX's MLPs use). The values agree with the reference's to a few
+// float32 ulp, which the rounding to 16 bits hides except next to a boundary,
+// but for the far negative tail: below x = -4 or so the reference's cancelling
+// float32 1 + erf / 1 + tanh sits on the 2^-24 grid, and below about -5.5 it
+// returns -0. There the values here are the accurate ones, so the 16-bit
+// results can differ from the reference's; those elements are below 1e-4 in
+// magnitude (codes 0 unless a whole row lies that far out).
 template <int ACT>
 __device__ __forceinline__ float act_f32(float x) {
   return ACT == DC_ACT_GELU_TANH ? gelu_tanh_f32(x) : gelu_erf_f32(x);

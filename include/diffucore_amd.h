@@ -52,7 +52,8 @@ int dc_quantize_rows(const void* x, int x_dtype, int64_t M, int64_t K, int64_t l
                      int8_t* q, int64_t ldq, float* scale, void* stream);
 
 /* Activations for dc_act_quantize_rows. */
-enum { DC_ACT_NONE = 0, DC_ACT_GELU_ERF = 1, DC_ACT_GELU_TANH = 2, DC_ACT_GEGLU = 3 };
+enum { DC_ACT_NONE = 0, DC_ACT_GELU_ERF = 1, DC_ACT_GELU_TANH = 2, DC_ACT_GEGLU = 3,
+       DC_ACT_SILU = 4, DC_ACT_QUICK_GELU = 5 };
 
 /*
  * dc_quantize_rows of the rows of concat(x1, act(x2)), in one pass:
@@ -378,6 +379,95 @@ int dc_int8_attn_fwd_noalloc(const void* q, const void* k, const void* v, void* 
  */
 int dc_int8_attn_quantize_q(const void* q, int dtype, int B, int H, int Lq, int D,
                             const int64_t q_strides[3], int8_t* q8, float* qs, void* stream);
+
+/*
+ * 16-bit feed-forward operators with their backward passes (fp16 / bf16, sums
+ * in float32). No counterpart in the reference, whose 16-bit layers run torch's
+ * own ops (nn.LayerNorm, nn.Linear, unet.py:148-165's x * F.gelu(gate)).
+ *
+ * Operands of the products (x, w, dz) are read 16 bytes at a time: pointers are
+ * 16-byte aligned, row strides multiples of 8 elements, and each row can be read
+ * up to its width rounded up to 8, where what lies past the width has to be 0 if
+ * products sum over it (said below). z, out, dy and the residual take any stride
+ * and alignment of their element. No output may overlap an input. `ws` is scratch of dc_linear16_workspace_bytes(op, M, N, K) bytes
+ * (op DC_LINEAR16_*), 16-byte aligned, NULL where that is 0; calls that overlap
+ * in time need scratch of their own. Results do not depend on timing: nothing
+ * is summed by atomics.
+ */
+enum { DC_LINEAR16_FWD = 0, DC_LINEAR16_GATED = 1, DC_LINEAR16_DX = 2, DC_LINEAR16_DX2 = 3,
+       DC_LINEAR16_DW = 4, DC_LINEAR16_DW2 = 5 };
+size_t dc_linear16_workspace_bytes(int op, int64_t M, int64_t N, int64_t K);
+
+/*
+ * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once; K % 8 == 0
+ * (a caller pads x and w with zeros). bias [N] of
+ * bias_dtype (DC_NONE: none), res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
+ * GELU_TANH / SILU / QUICK_GELU. z (or NULL) takes the pre-activation
+ * x w^T + bias for dc_act16_bwd, in float32.
+ */
+int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                const void* res, int64_t ldr, int act, void* out, int64_t ldo, float* z, int64_t ldz, int dtype,
+                int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * out[M, N] = (x wv^T + bv) * act(x wg^T + bg), both weights [N, K] (the two
+ * halves of a GEGLU projection, or matrices of their own), rounded once; zv and
+ * zg (both or neither NULL; one row stride) take the two pre-activations.
+ */
+int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg, int64_t ldwg, const void* bv,
+               const void* bg, int bias_dtype, int act, void* out, int64_t ldo, float* zv, float* zg, int64_t ldz,
+               int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * dx[M, K] = dz[M, N] w[N, K], plus dz2 w2 (dz2 with dz's row stride) where dz2
+ * is given. dz holds zeros in columns N .. N rounded up to 8, with a second term
+ * both do up to N rounded up to 64.
+ * op of its workspace: DC_LINEAR16_DX, or DX2 with the second term.
+ */
+int dc_linear16_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, const void* dz2,
+                   const void* w2, int64_t ldw2, void* dx, int64_t lddx, int dtype, int64_t M, int64_t N, int64_t K,
+                   void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * dw[N, K] = dz[M, N]^T x[M, K], and dw2 = dz2^T x in the same launch where
+ * dz2 is given (its strides those of dz and dw). op: DC_LINEAR16_DW, or DW2.
+ * M = 0 gives zeros.
+ */
+int dc_linear16_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, const void* dz2, void* dw, int64_t lddw,
+                   void* dw2, int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * The elementwise half of the backward passes, one read of its inputs:
+ *   dc_act16_bwd    dz = dy act'(z), db = column sums of dz before rounding
+ *   dc_gated16_bwd  dzv = dy act(zg), dzg = dy zv act'(zg), and their sums
+ * dz columns N .. N rounded up to 64 are set to 0 (row strides cover them; the
+ * dz pointers are 16-byte aligned). db / dbv / dbg ([N] of db_dtype) may be
+ * NULL; dc_act16_bwd with z and dz NULL sums dy alone. ws: dc_act16_bwd_workspace_bytes
+ * bytes when sums are asked for.
+ */
+size_t dc_act16_bwd_workspace_bytes(int64_t M, int64_t N, int gated);
+int dc_act16_bwd(const void* dy, int64_t lddy, const float* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db,
+                 int db_dtype, int dtype, int64_t M, int64_t N, void* ws, size_t ws_bytes, void* stream);
+int dc_gated16_bwd(const void* dy, int64_t lddy, const float* zv, const float* zg, int64_t ldz, int act, void* dzv,
+                   void* dzg, int64_t lddz, void* dbv, void* dbg, int db_dtype, int dtype, int64_t M, int64_t N,
+                   void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * y = (x - mean) rstd w + b over each row of D values, statistics in float32
+ * (two passes over registers: no cancellation), y rounded once. w, b [D] of
+ * w_dtype, each may be NULL. stats (float [2, M] or NULL) takes mean and rstd
+ * for the backward pass:
+ *   dxh = dy w, xh = (x - mean) rstd,
+ *   dx = rstd (dxh - mean(dxh) - xh mean(dxh xh)), dw = sum dy xh, db = sum dy.
+ * dx, dw and db may be NULL. Any D up to 2^24, rows at any stride and element
+ * alignment. ws: dc_layer_norm_bwd_workspace_bytes bytes, 16-byte aligned.
+ */
+int dc_layer_norm(const void* x, int64_t ldx, int x_dtype, const void* w, const void* b, int w_dtype, float eps,
+                  void* y, int64_t ldy, float* stats, int64_t M, int64_t D, void* stream);
+size_t dc_layer_norm_bwd_workspace_bytes(int64_t M, int64_t D, int x_dtype);
+int dc_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, int x_dtype, const void* w,
+                      int w_dtype, const float* stats, void* dx, int64_t lddx, void* dw, void* db, int64_t M,
+                      int64_t D, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * MFMA throughput calibration (no counterpart in the reference; measurement
