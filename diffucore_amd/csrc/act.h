@@ -121,20 +121,73 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 
 // ---------------------------------------------------------------- unaligned vectors
 
-// N consecutive 16-bit or 32-bit values whose address need only be aligned to
-// one element (rows of an odd width): the compiler still makes one wide access
-// of it, which global memory takes at any address on gfx950.
-struct __attribute__((packed, aligned(2))) U16x8 { uint32_t v[4]; };
-struct __attribute__((packed, aligned(4))) U32x4 { uint32_t v[4]; };
+// Wide accesses whose address need only be aligned to one element (rows of an
+// odd width): the compiler makes one access of each, which global memory takes
+// at any address on gfx950.
+template <class E, int N>
+struct __attribute__((packed, aligned(sizeof(E)))) AnyWords { uint32_t v[N]; };
 
-__device__ __forceinline__ uint4 load16_any(const uint16_t* p) {
-  const U16x8 u = *reinterpret_cast<const U16x8*>(p);
-  return make_uint4(u.v[0], u.v[1], u.v[2], u.v[3]);
+template <class E, int N>
+__device__ __forceinline__ AnyWords<E, N> load_words(const E* p) {
+  return *reinterpret_cast<const AnyWords<E, N>*>(p);
 }
-__device__ __forceinline__ void store16_any(uint16_t* p, uint4 v) {
-  U16x8 u;
-  u.v[0] = v.x, u.v[1] = v.y, u.v[2] = v.z, u.v[3] = v.w;
-  *reinterpret_cast<U16x8*>(p) = u;
+template <class E, int N>
+__device__ __forceinline__ void store_words(E* p, AnyWords<E, N> w) {
+  *reinterpret_cast<AnyWords<E, N>*>(p) = w;
+}
+
+// A 16-byte chunk of a row of which `n` elements are left: whole, or the row's
+// tail (the rest read as 0) in at most one access of each power of two.
+__device__ __forceinline__ uint4 load_chunk16(const uint16_t* p, int64_t n) {
+  if (n >= 8) {
+    const auto u = load_words<uint16_t, 4>(p);
+    return make_uint4(u.v[0], u.v[1], u.v[2], u.v[3]);
+  }
+  const int k = n > 0 ? (int)n : 0;
+  uint32_t a0 = 0u, a1 = 0u, b = 0u, c = 0u;
+  if (k & 4) {
+    const auto u = load_words<uint16_t, 2>(p);
+    a0 = u.v[0], a1 = u.v[1];
+  }
+  if (k & 2) b = load_words<uint16_t, 1>(p + (k & 4)).v[0];
+  if (k & 1) c = p[k & 6];
+  const uint32_t bc = k & 2 ? b : c, cz = k & 2 ? c : 0u;   // the words after the four
+  return k & 4 ? make_uint4(a0, a1, bc, cz) : make_uint4(bc, cz, 0u, 0u);
+}
+__device__ __forceinline__ void store_chunk16(uint16_t* p, int64_t n, uint4 v) {
+  if (n >= 8) {
+    store_words<uint16_t, 4>(p, {{v.x, v.y, v.z, v.w}});
+    return;
+  }
+  const int k = n > 0 ? (int)n : 0;
+  uint32_t bc = v.x, cz = v.y;
+  if (k & 4) {
+    store_words<uint16_t, 2>(p, {{v.x, v.y}});
+    bc = v.z, cz = v.w;
+  }
+  if (k & 2) store_words<uint16_t, 1>(p + (k & 4), {{bc}});
+  if (k & 1) p[k & 6] = (uint16_t)(k & 2 ? cz : bc);
+}
+__device__ __forceinline__ float4 load_chunk32(const float* p, int64_t n) {
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (n >= 4) {
+    const auto u = load_words<float, 4>(p);
+    return make_float4(__uint_as_float(u.v[0]), __uint_as_float(u.v[1]), __uint_as_float(u.v[2]),
+                       __uint_as_float(u.v[3]));
+  }
+  if (n > 0) f.x = p[0];
+  if (n > 1) f.y = p[1];
+  if (n > 2) f.z = p[2];
+  return f;
+}
+__device__ __forceinline__ void store_chunk32(float* p, int64_t n, float4 f) {
+  if (n >= 4) {
+    store_words<float, 4>(p, {{__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)}});
+    return;
+  }
+  if (n > 0) p[0] = f.x;
+  if (n > 1) p[1] = f.y;
+  if (n > 2) p[2] = f.z;
 }
 
 }  // namespace dc

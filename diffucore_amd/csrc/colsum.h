@@ -35,30 +35,18 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Up to 8 16-bit values from p (n of them, the rest 0), at any element alignment.
+// 8 values from p, of which n are left in the row (the rest 0), at any element alignment.
 template <int DT>
 __device__ __forceinline__ void load8_n(const uint16_t* p, int64_t n, float (&f)[8]) {
-  if (n >= 8) {
-    unpack8<DT>(load16_any(p), f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = e < n ? h16_to_f32<DT>(p[e]) : 0.0f;
-  }
+  unpack8<DT>(load_chunk16(p, n), f);
 }
-
-// Up to 8 floats from p (n of them, the rest 0), at any element alignment.
 __device__ __forceinline__ void load8_n(const float* p, int64_t n, float (&f)[8]) {
-  if (n >= 8) {
-#pragma unroll
-    for (int q = 0; q < 8; q += 4) {
-      const U32x4 u = *reinterpret_cast<const U32x4*>(p + q);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[q + e] = __uint_as_float(u.v[e]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = e < n ? p[e] : 0.0f;
-  }
+  const float4 a = load_chunk32(p, n), b = load_chunk32(p + 4, n - 4);
+  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+__device__ __forceinline__ void store8_n(float* p, int64_t n, const float (&f)[8]) {
+  store_chunk32(p, n, make_float4(f[0], f[1], f[2], f[3]));
+  store_chunk32(p + 4, n - 4, make_float4(f[4], f[5], f[6], f[7]));
 }
 
 }  // namespace dc

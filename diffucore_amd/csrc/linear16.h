@@ -122,32 +122,6 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// 8 outputs of row m from column n of an [M, N] matrix; the row's tail one by one.
-template <int DT>
-__device__ __forceinline__ void put16(uint16_t* row, int n, int N, uint4 v) {
-  if (n + 8 <= N) {
-    store16_any(row + n, v);
-  } else {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    for (int e = 0; e < 8 && n + e < N; ++e) row[n + e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-  }
-}
-__device__ __forceinline__ void put32(float* row, int n, int N, const float (&v)[8]) {
-  if (n + 8 <= N) {
-#pragma unroll
-    for (int q = 0; q < 8; q += 4) {
-      U32x4 u;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) u.v[e] = __float_as_uint(v[q + e]);
-      *reinterpret_cast<U32x4*>(row + n + q) = u;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (n + e < N) row[n + e] = v[e];
-  }
-}
-
 // One wave's FN x FM blocks leave through its share of the LDS ring, 32 rows at
 // a time, float32: put(row, chunk, v) gets 8 consecutive columns of one row
 // (chunk: which 8 of the 32 * FN), lanes along the row.
@@ -496,9 +470,10 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
       if (m >= p.M) return;
       if constexpr (GATED) {
         const int n = nb + c / 8 * 32 + c % 4 * 8;   // 4 chunks of values, then 4 of gates
-        put32(part + (int64_t)m * p.width + (c / 4 & 1) * p.N, n, p.N, v);
+        store8_n(part + (int64_t)m * p.width + (c / 4 & 1) * p.N + n, p.N - n, v);
       } else {
-        put32(part + (int64_t)m * p.width, nb + 8 * c, p.N, v);
+        const int n = nb + 8 * c;
+        store8_n(part + (int64_t)m * p.width + n, p.N - n, v);
       }
     });
     return;
@@ -523,8 +498,8 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
         if constexpr (GATED) g[e] += bg[e];
       }
       if (p.z) {
-        put32(p.z + (int64_t)m * p.ldz, n, p.N, v);
-        if constexpr (GATED) put32(p.z2 + (int64_t)m * p.ldz, n, p.N, g);
+        store8_n(p.z + (int64_t)m * p.ldz + n, p.N - n, v);
+        if constexpr (GATED) store8_n(p.z2 + (int64_t)m * p.ldz + n, p.N - n, g);
       }
       with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
         constexpr int ACT = decltype(act_)::value;
@@ -540,12 +515,13 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += s[e];
       }
-      put16<DT>(p.out + (int64_t)m * p.ldo, n, p.N, pack8<DT>(v));
+      store_chunk16(p.out + (int64_t)m * p.ldo + n, p.N - n, pack8<DT>(v));
     });
   } else {
     rows_h16<DT, FN, FM>(acc, share, lane, [&](int r, int c, uint4 v) __attribute__((always_inline)) {
       const int m = mb + r;
-      if (m < p.M) put16<DT>(p.out + (int64_t)m * p.ldo, nb + 8 * c, p.N, v);
+      const int n = nb + 8 * c;
+      if (m < p.M) store_chunk16(p.out + (int64_t)m * p.ldo + n, p.N - n, v);
     });
   }
 }
@@ -585,8 +561,8 @@ __global__ void __launch_bounds__(256) linear16_join_kernel(Gemm16 p) {
       if constexpr (GATED) g[e] += bias_at(p.bias2, p.bias_dtype, n + e);
     }
     if (p.z) {
-      put32(p.z + m * p.ldz, n, p.N, v);
-      if constexpr (GATED) put32(p.z2 + m * p.ldz, n, p.N, g);
+      store8_n(p.z + m * p.ldz + n, left, v);
+      if constexpr (GATED) store8_n(p.z2 + m * p.ldz + n, left, g);
     }
     with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
       constexpr int ACT = decltype(act_)::value;
@@ -603,7 +579,7 @@ __global__ void __launch_bounds__(256) linear16_join_kernel(Gemm16 p) {
       for (int e = 0; e < 8; ++e) v[e] += r[e];
     }
   }
-  put16<DT>((problem ? p.out2 : p.out) + m * p.ldo, n, p.N, pack8<DT>(v));
+  store_chunk16((problem ? p.out2 : p.out) + m * p.ldo + n, left, pack8<DT>(v));
 }
 
 // ---------------------------------------------------------------- launch
