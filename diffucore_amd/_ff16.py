@@ -20,6 +20,8 @@ HIP kernels, and raise where the library is missing.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -30,7 +32,7 @@ from . import _lib
 ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 4, "quick_gelu": 5}
 _HALF = (torch.float16, torch.bfloat16)
 _FLOAT = (torch.float16, torch.bfloat16, torch.float32)
-_FWD, _GATED, _DX, _DX2, _DW, _DW2 = range(6)
+_WANT_DX, _WANT_DW, _WANT_DW2, _WANT_DB = 1, 2, 4, 8   # DC_WANT_*
 
 
 def _act(z: torch.Tensor, act: str) -> torch.Tensor:
@@ -93,26 +95,15 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
     """``t`` as rows over its last dim, unit stride along it, rows that do not
     overlap (any row stride and alignment). A single row's stride is its
     length, whatever the tensor calls it."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    if (t.stride(1) != 1 and t.shape[1] != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    rows, width = t.shape
+    step, unit = t.stride()
+    if unit == 1 and step >= width:
+        return t
+    if (unit != 1 and width != 1) or (rows != 1 and step < width):
         t = t.contiguous()
-    if t.shape[0] == 1 or t.shape[1] == 1:
-        t = t.contiguous().view(t.shape)
-        if t.stride(0) != t.shape[1] or t.stride(1) != 1:
-            t = t.as_strided(t.shape, (t.shape[1], 1))
-    return t
-
-
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """``t [R, W]`` as an operand of the products: 16-byte aligned rows, zeros
-    up to a width that is a multiple of 8 (a copy where ``t`` has none)."""
-    t = _flat(t)
-    w = t.shape[1]
-    if w % 8:
-        return F.pad(t, (0, -w % 8))
-    if t.data_ptr() % 16 or (t.stride(0) % 8 and t.shape[0] > 1):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    return t.as_strided((rows, width), (width if rows == 1 else t.stride(0), 1))
 
 
 def _ptr(t):
@@ -131,9 +122,17 @@ def _scratch(nbytes: int, device):
     return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
 
 
-def _workspace(so, op: int, M: int, N: int, K: int, device):
-    n = so.dc_linear16_workspace_bytes(op, M, N, K)
-    return _scratch(n, device), n
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(query: str, device_index: int, *args) -> int:
+    """A workspace query on the current device (``device_index``), with each
+    pointer given as its offset in 16 bytes: a plain number per shape, the most
+    recent 1024 kept."""
+    return int(getattr(_lib.require(), query)(*args))
+
+
+def _at(t: torch.Tensor) -> int:
+    """``t``'s address as the workspace queries see it: its alignment."""
+    return 16 + t.data_ptr() % 16
 
 
 # ─── layer norm ──────────────────────────────────────────────────────────────
@@ -202,7 +201,9 @@ class _LayerNorm(torch.autograd.Function):
         dw = torch.empty(D, device=dev, dtype=ctx.param_dtype) if want_w else None
         db = torch.empty(D, device=dev, dtype=ctx.param_dtype) if want_b else None
         with _lib.device_ctx(dev):
-            need = so.dc_layer_norm_bwd_workspace_bytes(M, D, _code(x)) if want_w or want_b else 0
+            need = 0
+            if want_w or want_b:
+                need = _scratch_bytes("dc_layer_norm_bwd_workspace_bytes", dev.index, M, D, _code(x))
             ws = _scratch(need, dev)
             code = _lib.NONE if ctx.param_dtype is None else _lib.dtype_code(ctx.param_dtype)
             rc = so.dc_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), _code(x),
@@ -220,8 +221,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     ``x [..., K]``, ``weight [N, K]`` of one dtype (fp16 or bf16), ``bias [N]``
     of that dtype or float32, ``residual [..., N]`` of ``x``'s dtype. ``act`` is
     one of :data:`ACTIVATIONS` (``"gelu"`` the erf form, ``"quick_gelu"``
-    ``z * sigmoid(1.702 z)``). Any sizes; widths that are not multiples of 8
-    or rows that are not 16-byte aligned cost a padded copy of the operand."""
+    ``z * sigmoid(1.702 z)``). Any sizes; an operand whose width or row stride
+    is not a multiple of 8, or that is not 16-byte aligned, costs a padded copy."""
     what = "linear_act"
     code = _check_act(what, act)
     _check_product(what, x, weight)
@@ -241,7 +242,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
     so = _lib.require()
     dev, dt = x.device, _lib.dtype_code(x.dtype)
-    x2, w2 = _operand(x), _operand(weight)
+    x2, w2 = _flat(x), _flat(weight)
     (M, K), N = x2.shape, w2.shape[0]
     out = torch.empty((*x.shape[:-1], N), device=dev, dtype=x.dtype)
     if M == 0 or N == 0:
@@ -249,34 +250,15 @@ def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
     bias = _contig(bias)
     r2 = None if residual is None else _flat(residual)
     z = torch.empty((M, N), device=dev, dtype=torch.float32) if keep else None
+    ldx, ldw = x2.stride(0), w2.stride(0)
     with _lib.device_ctx(dev):
-        ws, need = _workspace(so, _FWD, M, N, K, dev)
-        rc = so.dc_linear16(x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), _ptr(bias), _code(bias),
-                            _ptr(r2), 0 if r2 is None else r2.stride(0), act, out.data_ptr(), N, _ptr(z), N, dt, M, N,
-                            K, _ptr(ws), need, _lib.stream_ptr(dev))
+        need = _scratch_bytes("dc_linear16_workspace_bytes", dev.index, _at(x2), ldx, _at(w2), ldw, M, N, K)
+        ws = _scratch(need, dev)
+        rc = so.dc_linear16(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(bias), _code(bias), _ptr(r2),
+                            0 if r2 is None else r2.stride(0), act, out.data_ptr(), N, _ptr(z), N, dt, M, N, K,
+                            _ptr(ws), need, _lib.stream_ptr(dev))
     _lib.check(rc, "dc_linear16")
     return out, z
-
-
-def _dx(so, dz, w, dz2, w2, M: int, N: int, x: torch.Tensor) -> torch.Tensor:
-    """``dz @ w (+ dz2 @ w2)`` in ``x``'s shape; ``dz`` and ``w`` are operands."""
-    dev, K = x.device, x.shape[-1]
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    ws, need = _workspace(so, _DX if dz2 is None else _DX2, M, N, K, dev)
-    rc = so.dc_linear16_dx(dz.data_ptr(), dz.stride(0), w.data_ptr(), w.stride(0), _ptr(dz2), _ptr(w2),
-                           0 if w2 is None else w2.stride(0), dx.data_ptr(), K, _lib.dtype_code(x.dtype), M, N, K,
-                           _ptr(ws), need, _lib.stream_ptr(dev))
-    _lib.check(rc, "dc_linear16_dx")
-    return dx
-
-
-def _dw(so, dz, x2, dz2, dw, dw2, M: int, N: int, K: int) -> None:
-    """``dw = dz.T @ x2`` (and ``dw2`` of ``dz2``); ``dz`` and ``x2`` are operands."""
-    dev = dz.device
-    ws, need = _workspace(so, _DW if dz2 is None else _DW2, M, N, K, dev)
-    rc = so.dc_linear16_dw(dz.data_ptr(), dz.stride(0), x2.data_ptr(), x2.stride(0), _ptr(dz2), dw.data_ptr(), K,
-                           _ptr(dw2), _lib.dtype_code(dz.dtype), M, N, K, _ptr(ws), need, _lib.stream_ptr(dev))
-    _lib.check(rc, "dc_linear16_dw")
 
 
 class _LinearAct(torch.autograd.Function):
@@ -293,34 +275,29 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
-        dx = dw = db = None
-        if want_x or want_w or want_b:
-            so, dev, dt = _lib.require(), x.device, _lib.dtype_code(x.dtype)
-            N, K = weight.shape
-            M = x.numel() // K
-            if M == 0 or N == 0:
-                return (torch.zeros_like(x) if want_x else None, torch.zeros_like(weight) if want_w else None,
-                        torch.zeros(N, device=dev, dtype=ctx.bias_dtype) if want_b else None,
-                        dy if want_r else None, None)
-            dy2 = _flat(dy)
-            with _lib.device_ctx(dev):
-                db = torch.empty(N, device=dev, dtype=ctx.bias_dtype) if want_b else None
-                pad = -(-N // 64) * 64
-                dz = torch.empty((M, pad), device=dev, dtype=x.dtype) if ctx.act else None
-                if dz is not None or want_b:
-                    need = so.dc_act16_bwd_workspace_bytes(M, N, 0) if want_b else 0
-                    ws = _scratch(need, dev)
-                    rc = so.dc_act16_bwd(dy2.data_ptr(), dy2.stride(0), _ptr(z), N, ctx.act, _ptr(dz), pad, _ptr(db),
-                                         _code(db), dt, M, N, _ptr(ws), need, _lib.stream_ptr(dev))
-                    _lib.check(rc, "dc_act16_bwd")
-                if dz is None and (want_x or want_w):
-                    dz = _operand(dy2)
-                if want_x:
-                    dx = _dx(so, dz, _operand(weight), None, None, M, N, x)
-                if want_w:
-                    dw = torch.empty((N, K), device=dev, dtype=x.dtype)
-                    _dw(so, dz, _operand(x), None, dw, None, M, N, K)
-        return dx, dw, db, dy if want_r else None, None
+        dres = dy if want_r else None
+        if not (want_x or want_w or want_b):
+            return None, None, None, dres, None
+        so, dev, dt = _lib.require(), x.device, x.dtype
+        N, K = weight.shape
+        dx = torch.empty(x.shape, device=dev, dtype=dt) if want_x else None
+        dw = torch.empty((N, K), device=dev, dtype=dt) if want_w else None
+        db = torch.empty(N, device=dev, dtype=ctx.bias_dtype) if want_b else None
+        M = x.numel() // K
+        if M == 0 or N == 0:
+            return (*(t if t is None else t.zero_() for t in (dx, dw, db)), dres, None)
+        dy2, x2, w2 = _flat(dy), _flat(x), _flat(weight)
+        ldy, ldx, ldw = dy2.stride(0), x2.stride(0), w2.stride(0)
+        want = want_x * _WANT_DX + want_w * _WANT_DW + want_b * _WANT_DB
+        with _lib.device_ctx(dev):
+            need = _scratch_bytes("dc_linear16_bwd_workspace_bytes", dev.index, _at(dy2), ldy, _at(x2), ldx, _at(w2),
+                                  ldw, ctx.act, want, M, N, K)
+            ws = _scratch(need, dev)
+            rc = so.dc_linear16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), N, ctx.act,
+                                    _ptr(dx), K, _ptr(dw), K, _ptr(db), _code(db), _lib.dtype_code(dt), M, N, K,
+                                    _ptr(ws), need, _lib.stream_ptr(dev))
+        _lib.check(rc, "dc_linear16_bwd")
+        return dx, dw, db, dres, None
 
 
 # ─── gated projection ────────────────────────────────────────────────────────
@@ -364,10 +341,10 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
 
 def _halves(weight, gate_weight):
-    """Value and gate weights ``[F, K]`` as operands, of one stacked weight or two."""
-    w = _operand(weight)
+    """Value and gate weights ``[F, K]``, of one stacked weight or two."""
+    w = _flat(weight)
     if gate_weight is not None:
-        return w, _operand(gate_weight)
+        return w, _flat(gate_weight)
     f = w.shape[0] // 2
     return w[:f], w[f:]
 
@@ -375,7 +352,7 @@ def _halves(weight, gate_weight):
 def _gated_forward(x, weight, bias, gate_weight, gate_bias, act: int, keep: bool):
     so = _lib.require()
     dev = x.device
-    x2 = _operand(x)
+    x2 = _flat(x)
     wv, wg = _halves(weight, gate_weight)
     (M, K), N = x2.shape, wv.shape[0]
     out = torch.empty((*x.shape[:-1], N), device=dev, dtype=x.dtype)
@@ -387,10 +364,13 @@ def _gated_forward(x, weight, bias, gate_weight, gate_bias, act: int, keep: bool
         bg = bv + N * bias.element_size()
     z = torch.empty((2, M, N), device=dev, dtype=torch.float32) if keep else None
     zv = _ptr(z)
+    ldx, ldv, ldg = x2.stride(0), wv.stride(0), wg.stride(0)
     with _lib.device_ctx(dev):
-        ws, need = _workspace(so, _GATED, M, N, K, dev)
-        rc = so.dc_gated16(x2.data_ptr(), x2.stride(0), wv.data_ptr(), wv.stride(0), wg.data_ptr(), wg.stride(0), bv,
-                           bg, _code(bias if bias is not None else gate_bias), act, out.data_ptr(), N, zv,
+        need = _scratch_bytes("dc_gated16_workspace_bytes", dev.index, _at(x2), ldx, _at(wv), ldv, _at(wg), ldg, M, N,
+                              K)
+        ws = _scratch(need, dev)
+        rc = so.dc_gated16(x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, bv, bg,
+                           _code(bias if bias is not None else gate_bias), act, out.data_ptr(), N, zv,
                            None if z is None else zv + M * N * 4, N, _lib.dtype_code(x.dtype), M, N, K, _ptr(ws), need,
                            _lib.stream_ptr(dev))
     _lib.check(rc, "dc_gated16")
@@ -410,49 +390,38 @@ class _GatedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, gate_weight, z = ctx.saved_tensors
         want_x, want_w, want_b, want_wg, want_bg, _ = ctx.needs_input_grad
-        so, dev, K = _lib.require(), x.device, x.shape[-1]
+        so, dev, dt, K = _lib.require(), x.device, x.dtype, x.shape[-1]
         fused = gate_weight is None
-        N = weight.shape[0] // 2 if fused else weight.shape[0]
+        rows = weight.shape[0]
+        N = rows // 2 if fused else rows
+        dx = torch.empty(x.shape, device=dev, dtype=dt) if want_x else None
+        dw = torch.empty((rows, K), device=dev, dtype=dt) if want_w else None
+        dwg = torch.empty((N, K), device=dev, dtype=dt) if want_wg else None
+        db = torch.empty(rows, device=dev, dtype=ctx.bias_dtype) if want_b else None
+        dbg = torch.empty(N, device=dev, dtype=ctx.bias_dtype) if want_bg else None
         M = x.numel() // K
-
-        def empty(want, *shape, dtype=x.dtype):
-            return torch.empty(shape, device=dev, dtype=dtype) if want else None
-
-        rows = 2 * N if fused else N
-        dw, dwg = empty(want_w, rows, K), empty(want_wg, N, K)
-        db, dbg = empty(want_b, rows, dtype=ctx.bias_dtype), empty(want_bg, N, dtype=ctx.bias_dtype)
         if M == 0 or N == 0:
-            for t in (dw, dwg, db, dbg):
-                if t is not None:
-                    t.zero_()
-            return torch.zeros_like(x) if want_x else None, dw, db, dwg, dbg, None
-        dy2, pad = _flat(dy), -(-N // 64) * 64
-        dz = torch.empty((2, M, pad), device=dev, dtype=x.dtype)
+            return (*(t if t is None else t.zero_() for t in (dx, dw, db, dwg, dbg)), None)
+        dy2, x2 = _flat(dy), _flat(x)
+        wv, wg = _halves(weight, gate_weight)
+        ldy, ldx, ldv, ldg = dy2.stride(0), x2.stride(0), wv.stride(0), wg.stride(0)
+        dwv_p, dwg_p, dbv_p, dbg_p = _ptr(dw), _ptr(dwg), _ptr(db), _ptr(dbg)
+        if fused and want_w:
+            dwg_p = dwv_p + N * K * dw.element_size()
+        if fused and want_b:
+            dbg_p = dbv_p + N * db.element_size()
+        want = (want_x * _WANT_DX + want_w * _WANT_DW + (want_w if fused else want_wg) * _WANT_DW2
+                + (want_b or want_bg) * _WANT_DB)
+        zv = z.data_ptr()
         with _lib.device_ctx(dev):
-            sums = want_b or want_bg
-            need = so.dc_act16_bwd_workspace_bytes(M, N, 1) if sums else 0
+            need = _scratch_bytes("dc_gated16_bwd_workspace_bytes", dev.index, _at(dy2), ldy, _at(x2), ldx, _at(wv), ldv,
+                                  _at(wg), ldg, want, M, N, K)
             ws = _scratch(need, dev)
-            dbv, dbg_p = _ptr(db), _ptr(dbg)
-            if fused and want_b:
-                dbg_p = dbv + N * db.element_size()
-            zv, dzv = z.data_ptr(), dz.data_ptr()
-            rc = so.dc_gated16_bwd(dy2.data_ptr(), dy2.stride(0), zv, zv + M * N * 4, N, ctx.act, dzv,
-                                   dzv + M * pad * 2, pad, dbv, dbg_p,
-                                   _lib.dtype_code(ctx.bias_dtype) if sums else _lib.NONE, _lib.dtype_code(x.dtype),
-                                   M, N, _ptr(ws), need, _lib.stream_ptr(dev))
-            _lib.check(rc, "dc_gated16_bwd")
-            dx = None
-            if want_x:
-                wv, wg = _halves(weight, gate_weight)
-                dx = _dx(so, dz[0], wv, dz[1], wg, M, N, x)
-            if want_w or want_wg:
-                x2 = _operand(x)
-                if fused:
-                    _dw(so, dz[0], x2, dz[1], dw[:N], dw[N:], M, N, K)
-                elif want_w and want_wg:
-                    _dw(so, dz[0], x2, dz[1], dw, dwg, M, N, K)
-                else:
-                    _dw(so, dz[0] if want_w else dz[1], x2, None, dw if want_w else dwg, None, M, N, K)
+            rc = so.dc_gated16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, zv,
+                                   zv + M * N * 4, N, ctx.act, _ptr(dx), K, dwv_p, dwg_p, K, dbv_p, dbg_p,
+                                   _lib.NONE if ctx.bias_dtype is None else _lib.dtype_code(ctx.bias_dtype),
+                                   _lib.dtype_code(dt), M, N, K, _ptr(ws), need, _lib.stream_ptr(dev))
+        _lib.check(rc, "dc_gated16_bwd")
         return dx, dw, db, dwg, dbg, None
 
 

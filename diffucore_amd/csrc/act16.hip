@@ -28,7 +28,7 @@ struct ActBwdArgs {
   uint16_t* dg;
   float* part;          // [P][1 or 2][N], NULL: no sums
   int64_t lddy, ldz, lddz;
-  int M, N, pad;        // pad: columns of dz to fill (N rounded up to 64)
+  int M, N, pad;        // pad: columns of dz to fill (its row stride)
   int tx_log, rows;     // log2 TX; rows per workgroup
   int act;
 };
@@ -142,7 +142,7 @@ static ActBwdPlan act_bwd_plan(int64_t M, int64_t N) {
   ActBwdPlan r;
   r.tx_log = 0;
   while (r.tx_log < 6 && (8LL << r.tx_log) < N) ++r.tx_log;
-  const int64_t pad = (N + 63) / 64 * 64, TY = 256 >> r.tx_log;
+  const int64_t pad = (N + 63) / 64 * 64, TY = 256 >> r.tx_log;   // the columns of dz
   r.col_blocks = (int)((pad + (8LL << r.tx_log) - 1) / (8LL << r.tx_log));
   const int64_t most = (M + 4 * TY - 1) / (4 * TY);
   int64_t want = (8LL * device_cus() + r.col_blocks - 1) / r.col_blocks;
@@ -156,97 +156,50 @@ static ActBwdPlan act_bwd_plan(int64_t M, int64_t N) {
   return r;
 }
 
+size_t act16_bwd_part_bytes(int64_t M, int64_t N, bool gated) {
+  const ActBwdPlan r = act_bwd_plan(M, N);
+  return sizeof(float) * (size_t)r.row_blocks * (gated ? 2 : 1) * (size_t)N;
+}
+
 template <int MODE>
-static int run_act_bwd(const char* who, ActBwdArgs p, int dtype, void* db0, void* db1, int db_dtype, void* ws,
-                       size_t ws_bytes, hipStream_t st) {
+static int run_act_bwd(const char* who, ActBwdArgs p, int dtype, void* db0, void* db1, int db_dtype, hipStream_t st) {
   const ActBwdPlan r = act_bwd_plan(p.M, p.N);
-  const bool sums = db0 || db1;
-  if (sums) {
-    const size_t need = dc_act16_bwd_workspace_bytes(p.M, p.N, MODE == 2);
-    if (ws_bytes < need || !ws || !aligned16(ws)) {
-      set_error("%s: workspace too small or not 16-byte aligned (needs %zu bytes)", who, need);
-      return DC_EWORKSPACE;
-    }
-    p.part = static_cast<float*>(ws);
-  }
   p.tx_log = r.tx_log, p.rows = r.rows;
   const dim3 grid(r.col_blocks, r.row_blocks);
   if (dtype == DC_BF16) hipLaunchKernelGGL((act_bwd_kernel<DC_BF16, MODE>), grid, dim3(256), 0, st, p);
   else hipLaunchKernelGGL((act_bwd_kernel<DC_F16, MODE>), grid, dim3(256), 0, st, p);
   if (int e = launch_status(who)) return e;
-  return sums ? reduce_partials(p.part, r.row_blocks, MODE == 2 ? 2 : 1, p.N, db0, db1, db_dtype, st, who) : DC_OK;
+  return p.part ? reduce_partials(p.part, r.row_blocks, MODE == 2 ? 2 : 1, p.N, db0, db1, db_dtype, st, who) : DC_OK;
 }
 
-static int check_act_bwd(const char* who, int act, int dtype, int64_t M, int64_t N, int64_t lddy, bool sums,
-                         int db_dtype) {
-  const char* msg = nullptr;
-  if (M < 0 || N < 0 || M > 0x7fffffff || N > 0x7fffffc0) msg = "bad M/N";
-  else if (dtype != DC_F16 && dtype != DC_BF16) msg = "dtype must be DC_F16 or DC_BF16";
-  else if (act != DC_ACT_NONE && act != DC_ACT_GELU_ERF && act != DC_ACT_GELU_TANH && act != DC_ACT_SILU &&
-           act != DC_ACT_QUICK_GELU) msg = "bad act";
-  else if (lddy < N) msg = "lddy < N";
-  else if (sums && !float_dtype(db_dtype)) msg = "db_dtype must be DC_F16, DC_BF16 or DC_F32";
-  if (!msg) return DC_OK;
-  set_error("%s: %s", who, msg);
-  return DC_EINVAL;
+int act16_bwd(const char* who, const ActBwd& a, hipStream_t st) {
+  ActBwdArgs p{};
+  p.dy = static_cast<const uint16_t*>(a.dy), p.lddy = a.lddy, p.M = (int)a.M, p.N = (int)a.N;
+  p.za = a.zv, p.zg = a.zg, p.ldz = a.ldz, p.act = a.act;
+  p.da = static_cast<uint16_t*>(a.dzv), p.dg = static_cast<uint16_t*>(a.dzg), p.lddz = a.lddz, p.pad = (int)a.lddz;
+  p.part = a.dbv || a.dbg ? a.part : nullptr;
+  if (a.zg) return run_act_bwd<2>(who, p, a.dtype, a.dbv, a.dbg, a.db_dtype, st);
+  if (a.zv) return run_act_bwd<1>(who, p, a.dtype, a.dbv, nullptr, a.db_dtype, st);
+  return run_act_bwd<0>(who, p, a.dtype, a.dbv, nullptr, a.db_dtype, st);
+}
+
+// ---------------------------------------------------------------- padded copies
+
+// dst [M, W rounded up to 8] = src [M, W] and zeros: a thread a chunk of 8.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t M,
+                                                       int W) {
+  const int64_t chunks = (W + 7) / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * chunks) return;
+  const int64_t r = i / chunks, c = i % chunks;
+  *reinterpret_cast<uint4*>(dst + 8 * i) = load_chunk16(src + r * lds + 8 * c, W - 8 * c);
+}
+
+int pad_rows16(const char* who, const void* src, int64_t lds, void* dst, int64_t M, int64_t W, hipStream_t st) {
+  const int64_t n = M * ((W + 7) / 8);
+  if (n > 0x7fffffffLL * 256) return fail(DC_EINVAL, "pad_rows16: operand too large");
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
+                     static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), M, (int)W);
+  return launch_status(who);
 }
 
 }  // namespace dc
-
-using namespace dc;
-
-extern "C" size_t dc_act16_bwd_workspace_bytes(int64_t M, int64_t N, int gated) {
-  if (M <= 0 || N <= 0 || M > 0x7fffffff || N > 0x7fffffc0) return 0;
-  const ActBwdPlan r = act_bwd_plan(M, N);
-  return sizeof(float) * (size_t)r.row_blocks * (gated ? 2 : 1) * (size_t)N;
-}
-
-static bool bad_dz(const void* p, int64_t ldd, int64_t N) {
-  return !p || !aligned16(p) || ldd % 8 || ldd < (N + 63) / 64 * 64;
-}
-
-extern "C" int dc_act16_bwd(const void* dy, int64_t lddy, const float* z, int64_t ldz, int act, void* dz, int64_t lddz,
-                            void* db, int db_dtype, int dtype, int64_t M, int64_t N, void* ws, size_t ws_bytes,
-                            void* stream) {
-  clear_error();
-  if (int e = check_act_bwd("dc_act16_bwd", act, dtype, M, N, lddy, db != nullptr, db_dtype)) return e;
-  if (N == 0) return DC_OK;
-  if (M == 0)   // a sum over no rows
-    return db ? reduce_partials(nullptr, 0, 1, N, db, nullptr, db_dtype, (hipStream_t)stream, "dc_act16_bwd") : DC_OK;
-  if (!dy) return fail(DC_EINVAL, "dc_act16_bwd: null dy");
-  if (!z != !dz) return fail(DC_EINVAL, "dc_act16_bwd: z and dz go together");
-  ActBwdArgs p{};
-  p.dy = static_cast<const uint16_t*>(dy), p.lddy = lddy, p.M = (int)M, p.N = (int)N;
-  p.pad = (int)((N + 63) / 64 * 64), p.act = act;
-  if (!z) {
-    if (!db) return DC_OK;
-    return run_act_bwd<0>("dc_act16_bwd", p, dtype, db, nullptr, db_dtype, ws, ws_bytes, (hipStream_t)stream);
-  }
-  if (ldz < N) return fail(DC_EINVAL, "dc_act16_bwd: ldz < N");
-  if (bad_dz(dz, lddz, N))
-    return fail(DC_EUNSUPPORTED, "dc_act16_bwd: dz needs 16-byte aligned rows of at least N rounded up to 64");
-  p.za = z, p.ldz = ldz;
-  p.da = static_cast<uint16_t*>(dz), p.lddz = lddz;
-  return run_act_bwd<1>("dc_act16_bwd", p, dtype, db, nullptr, db_dtype, ws, ws_bytes, (hipStream_t)stream);
-}
-
-extern "C" int dc_gated16_bwd(const void* dy, int64_t lddy, const float* zv, const float* zg, int64_t ldz, int act,
-                              void* dzv, void* dzg, int64_t lddz, void* dbv, void* dbg, int db_dtype, int dtype,
-                              int64_t M, int64_t N, void* ws, size_t ws_bytes, void* stream) {
-  clear_error();
-  if (int e = check_act_bwd("dc_gated16_bwd", act, dtype, M, N, lddy, dbv || dbg, db_dtype)) return e;
-  if (N == 0) return DC_OK;
-  if (M == 0)
-    return dbv || dbg ? reduce_partials(nullptr, 0, 2, N, dbv, dbg, db_dtype, (hipStream_t)stream, "dc_gated16_bwd")
-                      : DC_OK;
-  if (!dy || !zv || !zg) return fail(DC_EINVAL, "dc_gated16_bwd: null pointer");
-  if (ldz < N) return fail(DC_EINVAL, "dc_gated16_bwd: ldz < N");
-  if (bad_dz(dzv, lddz, N) || bad_dz(dzg, lddz, N))
-    return fail(DC_EUNSUPPORTED, "dc_gated16_bwd: dz needs 16-byte aligned rows of at least N rounded up to 64");
-  ActBwdArgs p{};
-  p.dy = static_cast<const uint16_t*>(dy), p.lddy = lddy, p.M = (int)M, p.N = (int)N;
-  p.pad = (int)((N + 63) / 64 * 64), p.act = act;
-  p.za = zv, p.zg = zg, p.ldz = ldz;
-  p.da = static_cast<uint16_t*>(dzv), p.dg = static_cast<uint16_t*>(dzg), p.lddz = lddz;
-  return run_act_bwd<2>("dc_gated16_bwd", p, dtype, dbv, dbg, db_dtype, ws, ws_bytes, (hipStream_t)stream);
-}

@@ -11,6 +11,29 @@ namespace dc {
 int reduce_partials(const float* part, int P, int sections, int64_t width, void* out0, void* out1, int out_dtype,
                     hipStream_t st, const char* what);
 
+// The elementwise half of a feed-forward backward pass: dz of dy and the
+// pre-activations (zg: gated; neither: none), rows of lddz = N rounded up to 64
+// with zeros past N, and the sums of dz over rows before rounding (NULL: not
+// asked for). `part`: act16_bwd_part_bytes of scratch for the sums.
+struct ActBwd {
+  const void* dy;
+  int64_t lddy;
+  const float *zv, *zg;
+  int64_t ldz;
+  int act;
+  void *dzv, *dzg;
+  int64_t lddz;
+  void *dbv, *dbg;
+  int db_dtype, dtype;
+  int64_t M, N;
+  float* part;
+};
+int act16_bwd(const char* who, const ActBwd& a, hipStream_t st);
+size_t act16_bwd_part_bytes(int64_t M, int64_t N, bool gated);
+
+// dst [M, W rounded up to 8] (16-byte aligned) = src [M, W] and zeros.
+int pad_rows16(const char* who, const void* src, int64_t lds, void* dst, int64_t M, int64_t W, hipStream_t st);
+
 inline bool float_dtype(int dt) { return dt == DC_F16 || dt == DC_BF16 || dt == DC_F32; }
 
 // 8 consecutive 16-bit values as floats.

@@ -633,15 +633,44 @@ inline size_t plan16_bytes(const Plan16& plan, int64_t M, int64_t rows, int prob
   return plan.splits > 1 ? sizeof(float) * (size_t)plan.splits * problems * (size_t)M * (size_t)rows : 0;
 }
 
-int refuse(int code, const char* who, const char* msg);
-int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K);
-int check_scratch(const char* who, size_t need, const void* ws, size_t ws_bytes);
-
 inline int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// A product's operand: `width` contiguous values a row.
-inline bool bad_operand(const void* p, int64_t ld, int64_t width) {
-  return !aligned16(p) || ld % 8 || ld < width || ld >= (1 << 22);
+// A matrix argument: `rows` x `width` values of unit stride along a row.
+struct Mat16 {
+  const void* p;
+  int64_t ld, rows, width;
+};
+// Whether the product kernels can read it in place: 16-byte chunks of whole
+// rows, at 32-bit offsets within a tile. Otherwise it is copied to scratch.
+inline bool in_place(const Mat16& m) {
+  return aligned16(m.p) && m.ld % 8 == 0 && m.width % 8 == 0 && m.ld < (1 << 22);
 }
+
+// Hands out a call's scratch in 256-byte steps; with no base, only measures it.
+struct Scratch16 {
+  uint8_t* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    uint8_t* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+  // the operand as the kernels read it: itself, or room for its padded copy
+  Mat16 operand(const Mat16& m) {
+    if (in_place(m)) return m;
+    const int64_t w8 = round_up(m.width, 8);
+    return {take(2 * (size_t)m.rows * (size_t)w8), w8, m.rows, w8};
+  }
+};
+// Fills an operand's padded copy, if it has one.
+inline int pad_operand(const char* who, const Mat16& from, const Mat16& to, hipStream_t st) {
+  if (to.p == from.p || from.rows == 0) return DC_OK;
+  return pad_rows16(who, from.p, from.ld, const_cast<void*>(to.p), from.rows, from.width, st);
+}
+
+int refuse(int code, const char* who, const char* msg);
+// What every product checks: sizes, type, activation.
+int check_product(const char* who, int dtype, int act, int64_t M, int64_t N, int64_t K);
+int check_scratch(const char* who, size_t need, const void* ws, size_t ws_bytes);
 
 }  // namespace dc

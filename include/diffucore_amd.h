@@ -385,26 +385,25 @@ int dc_int8_attn_quantize_q(const void* q, int dtype, int B, int H, int Lq, int 
  * in float32). No counterpart in the reference, whose 16-bit layers run torch's
  * own ops (nn.LayerNorm, nn.Linear, unet.py:148-165's x * F.gelu(gate)).
  *
- * Operands of the products (x, w, dz) are read 16 bytes at a time: pointers are
- * 16-byte aligned, row strides multiples of 8 elements, and each row can be read
- * up to its width rounded up to 8, where what lies past the width has to be 0 if
- * products sum over it (said below). z, out, dy and the residual take any stride
- * and alignment of their element. No output may overlap an input. `ws` is scratch of dc_linear16_workspace_bytes(op, M, N, K) bytes
- * (op DC_LINEAR16_*), 16-byte aligned, NULL where that is 0; calls that overlap
- * in time need scratch of their own. Results do not depend on timing: nothing
- * is summed by atomics.
+ * Matrices have unit stride along their rows and any row stride of at least
+ * their width; pointers are aligned to their element. x, w and dy whose pointer
+ * is not 16-byte aligned, whose row stride or width is not a multiple of 8, or
+ * whose row stride is 2^22 or more are copied (padded) to scratch first; the
+ * workspace queries take the same pointers and strides as the call and say how
+ * much that, split-K sums and the backward's dz need. `ws` is 16-byte aligned;
+ * calls that overlap in time need scratch of their own. M < 2^30, N < 2^29,
+ * 0 < K < 2^22. No output may overlap an input. Results do not depend on
+ * timing: nothing is summed by atomics.
  */
-enum { DC_LINEAR16_FWD = 0, DC_LINEAR16_GATED = 1, DC_LINEAR16_DX = 2, DC_LINEAR16_DX2 = 3,
-       DC_LINEAR16_DW = 4, DC_LINEAR16_DW2 = 5 };
-size_t dc_linear16_workspace_bytes(int op, int64_t M, int64_t N, int64_t K);
 
 /*
- * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once; K % 8 == 0
- * (a caller pads x and w with zeros). bias [N] of
+ * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once. bias [N] of
  * bias_dtype (DC_NONE: none), res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
  * GELU_TANH / SILU / QUICK_GELU. z (or NULL) takes the pre-activation
- * x w^T + bias for dc_act16_bwd, in float32.
+ * x w^T + bias for dc_linear16_bwd, in float32.
  */
+size_t dc_linear16_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N,
+                                   int64_t K);
 int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
                 const void* res, int64_t ldr, int act, void* out, int64_t ldo, float* z, int64_t ldz, int dtype,
                 int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
@@ -414,43 +413,34 @@ int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
  * halves of a GEGLU projection, or matrices of their own), rounded once; zv and
  * zg (both or neither NULL; one row stride) take the two pre-activations.
  */
+size_t dc_gated16_workspace_bytes(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg,
+                                  int64_t ldwg, int64_t M, int64_t N, int64_t K);
 int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg, int64_t ldwg, const void* bv,
                const void* bg, int bias_dtype, int act, void* out, int64_t ldo, float* zv, float* zg, int64_t ldz,
                int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 
 /*
- * dx[M, K] = dz[M, N] w[N, K], plus dz2 w2 (dz2 with dz's row stride) where dz2
- * is given. dz holds zeros in columns N .. N rounded up to 8, with a second term
- * both do up to N rounded up to 64.
- * op of its workspace: DC_LINEAR16_DX, or DX2 with the second term.
+ * Gradients of dc_linear16 and dc_gated16, each output NULL where it is not
+ * wanted (`want` in the queries: DC_WANT_* of those that are):
+ *   dz = dy act'(z) (dz = dy for DC_ACT_NONE, where z is not read)
+ *   dzv = dy act(zg), dzg = dy zv act'(zg)
+ *   dx = dz w, dw = dz^T x, db = column sums of dz before it is rounded to
+ *   16 bits as the products' operand (the residual's gradient is dy itself).
+ * db / dbv / dbg are [N] of db_dtype. M = 0 gives zeros for dw and db.
  */
-int dc_linear16_dx(const void* dz, int64_t lddz, const void* w, int64_t ldw, const void* dz2,
-                   const void* w2, int64_t ldw2, void* dx, int64_t lddx, int dtype, int64_t M, int64_t N, int64_t K,
-                   void* ws, size_t ws_bytes, void* stream);
-
-/*
- * dw[N, K] = dz[M, N]^T x[M, K], and dw2 = dz2^T x in the same launch where
- * dz2 is given (its strides those of dz and dw). op: DC_LINEAR16_DW, or DW2.
- * M = 0 gives zeros.
- */
-int dc_linear16_dw(const void* dz, int64_t lddz, const void* x, int64_t ldx, const void* dz2, void* dw, int64_t lddw,
-                   void* dw2, int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
-
-/*
- * The elementwise half of the backward passes, one read of its inputs:
- *   dc_act16_bwd    dz = dy act'(z), db = column sums of dz before rounding
- *   dc_gated16_bwd  dzv = dy act(zg), dzg = dy zv act'(zg), and their sums
- * dz columns N .. N rounded up to 64 are set to 0 (row strides cover them; the
- * dz pointers are 16-byte aligned). db / dbv / dbg ([N] of db_dtype) may be
- * NULL; dc_act16_bwd with z and dz NULL sums dy alone. ws: dc_act16_bwd_workspace_bytes
- * bytes when sums are asked for.
- */
-size_t dc_act16_bwd_workspace_bytes(int64_t M, int64_t N, int gated);
-int dc_act16_bwd(const void* dy, int64_t lddy, const float* z, int64_t ldz, int act, void* dz, int64_t lddz, void* db,
-                 int db_dtype, int dtype, int64_t M, int64_t N, void* ws, size_t ws_bytes, void* stream);
-int dc_gated16_bwd(const void* dy, int64_t lddy, const float* zv, const float* zg, int64_t ldz, int act, void* dzv,
-                   void* dzg, int64_t lddz, void* dbv, void* dbg, int db_dtype, int dtype, int64_t M, int64_t N,
-                   void* ws, size_t ws_bytes, void* stream);
+enum { DC_WANT_DX = 1, DC_WANT_DW = 2, DC_WANT_DW2 = 4, DC_WANT_DB = 8 };
+size_t dc_linear16_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
+                                       int64_t ldw, int act, int want, int64_t M, int64_t N, int64_t K);
+int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                    const float* z, int64_t ldz, int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
+                    int db_dtype, int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+size_t dc_gated16_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* wv,
+                                      int64_t ldwv, const void* wg, int64_t ldwg, int want, int64_t M, int64_t N,
+                                      int64_t K);
+int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* wv, int64_t ldwv,
+                   const void* wg, int64_t ldwg, const float* zv, const float* zg, int64_t ldz, int act, void* dx,
+                   int64_t lddx, void* dwv, void* dwg, int64_t lddw, void* dbv, void* dbg, int db_dtype, int dtype,
+                   int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * y = (x - mean) rstd w + b over each row of D values, statistics in float32

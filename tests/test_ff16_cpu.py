@@ -5,8 +5,6 @@ return before any launch)."""
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 import torch.nn as nn
@@ -172,17 +170,20 @@ def _linear(x=P, ldx=64, w=P, ldw=64, bias=None, bdt=-1, res=None, ldr=0, act=0,
 
 
 def _gated(x=P, ldx=64, wv=P, wg=P, ldw=64, bv=None, bg=None, bdt=-1, act=1, out=P, ldo=32, zv=None, zg=None, ldz=0,
-           dt=0, M=4, N=32, K=64):
-    return _rc("dc_gated16", x, ldx, wv, ldw, wg, ldw, bv, bg, bdt, act, out, ldo, zv, zg, ldz, dt, M, N, K, None, 0,
+           dt=0, M=4, N=32, K=64, ws=None, n=0):
+    return _rc("dc_gated16", x, ldx, wv, ldw, wg, ldw, bv, bg, bdt, act, out, ldo, zv, zg, ldz, dt, M, N, K, ws, n, None)
+
+
+def _lbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, z=P, ldz=32, act=1, dx=P, lddx=64, dw=P, lddw=64, db=P, ddt=0, dt=1,
+          M=4, N=32, K=64, ws=P, n=1 << 30):
+    return _rc("dc_linear16_bwd", dy, ldy, x, ldx, w, ldw, z, ldz, act, dx, lddx, dw, lddw, db, ddt, dt, M, N, K, ws, n,
                None)
 
 
-def _dx(dz=P, ldz=64, w=P, ldw=64, dz2=None, w2=None, dx=P, lddx=64, dt=1, M=4, N=64, K=64):
-    return _rc("dc_linear16_dx", dz, ldz, w, ldw, dz2, w2, ldw, dx, lddx, dt, M, N, K, None, 0, None)
-
-
-def _dw(dz=P, ldz=64, x=P, ldx=64, dz2=None, dw=P, lddw=64, dw2=None, dt=1, M=4, N=64, K=64):
-    return _rc("dc_linear16_dw", dz, ldz, x, ldx, dz2, dw, lddw, dw2, dt, M, N, K, None, 0, None)
+def _gbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, wg=P, zv=P, zg=P, ldz=32, act=1, dx=P, lddx=64, dw=P, dwg=P, lddw=64,
+          db=P, dbg=P, ddt=0, dt=1, M=4, N=32, K=64, ws=P, n=1 << 30):
+    return _rc("dc_gated16_bwd", dy, ldy, x, ldx, w, ldw, wg, ldw, zv, zg, ldz, act, dx, lddx, dw, dwg, lddw, db, dbg,
+               ddt, dt, M, N, K, ws, n, None)
 
 
 def _norm(x=P, ldx=8, xdt=0, w=None, b=None, wdt=-1, y=P, ldy=8, stats=None, M=4, D_=8):
@@ -190,22 +191,29 @@ def _norm(x=P, ldx=8, xdt=0, w=None, b=None, wdt=-1, y=P, ldy=8, stats=None, M=4
 
 
 @pytest.mark.parametrize("call, kw, code, match", [
-    (_linear, dict(M=-1), 1, "negative"), (_linear, dict(N=1 << 31), 1, "too large"), (_linear, dict(dt=2), 1, "dtype"),
-    (_linear, dict(act=3), 1, "act"), (_linear, dict(K=0), 1, "K must be"), (_linear, dict(x=None), 1, "null"),
-    (_linear, dict(out=None), 1, "null"), (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"),
-    (_linear, dict(ldo=31), 1, "stride"), (_linear, dict(res=P, ldr=8), 1, "stride"),
-    (_linear, dict(z=P, ldz=8), 1, "stride"), (_linear, dict(K=60), 2, "multiples of 8"),
-    (_linear, dict(ldx=68), 2, "multiples of 8"), (_linear, dict(x=P + 8), 2, "aligned"),
-    (_linear, dict(ldw=56), 2, "aligned"), (_linear, dict(M=0, x=None), 0, ""), (_linear, dict(N=0, K=0), 0, ""),
+    (_linear, dict(M=-1), 1, "bad M/N/K"), (_linear, dict(M=1 << 30), 1, "too large"),
+    (_linear, dict(N=1 << 29), 1, "too large"), (_linear, dict(K=1 << 22, ldx=1 << 22), 1, "too large"),
+    (_linear, dict(dt=2), 1, "dtype"), (_linear, dict(act=3), 1, "act"), (_linear, dict(K=0), 1, "bad M/N/K"),
+    (_linear, dict(x=None), 1, "null"), (_linear, dict(out=None), 1, "null"),
+    (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"), (_linear, dict(ldo=31), 1, "stride"),
+    (_linear, dict(res=P, ldr=8), 1, "stride"), (_linear, dict(z=P, ldz=8), 1, "stride"),
+    (_linear, dict(ldx=63), 1, "stride"), (_linear, dict(ldw=56), 1, "stride"),
+    (_linear, dict(K=60, ldx=60, ldw=60), 4, "needs"), (_linear, dict(ldx=68), 4, "needs"),
+    (_linear, dict(x=P + 8), 4, "needs"), (_linear, dict(x=P + 8, ws=P + 8, n=1 << 20), 4, "aligned"),
+    (_linear, dict(M=0, x=None), 0, ""), (_linear, dict(N=0), 0, ""),
     (_gated, dict(wg=None), 1, "null"), (_gated, dict(act=3), 1, "act"), (_gated, dict(zv=P, ldz=32), 1, "together"),
-    (_gated, dict(bg=P, bdt=-1), 1, "bias_dtype"), (_gated, dict(wg=P + 2), 2, "aligned"),
-    (_gated, dict(M=0), 0, ""), (_gated, dict(K=0), 1, "K must be"), (_gated, dict(dt=2), 1, "dtype"),
-    (_dx, dict(dz2=P), 1, "null"), (_dx, dict(N=0), 1, "N must be"), (_dx, dict(lddx=60), 1, "stride"),
-    (_dx, dict(N=60, ldz=56), 2, "cover"), (_dx, dict(N=60, ldz=64, dz2=P, w2=P + 8), 2, "cover"),
-    (_dx, dict(N=70, ldz=72, dz2=P, w2=P), 2, "cover"), (_dx, dict(K=60, lddx=60, ldw=56), 2, "cover"),
-    (_dx, dict(M=0), 0, ""), (_dx, dict(K=0), 0, ""),
-    (_dw, dict(dz2=P), 1, "null"), (_dw, dict(dw=None), 1, "null"), (_dw, dict(lddw=8), 1, "stride"),
-    (_dw, dict(N=66, ldz=64), 2, "cover"), (_dw, dict(x=P + 4), 2, "cover"), (_dw, dict(N=0), 0, ""),
+    (_gated, dict(bg=P, bdt=-1), 1, "bias_dtype"), (_gated, dict(wg=P + 2), 4, "needs"),
+    (_gated, dict(M=0), 0, ""), (_gated, dict(K=0), 1, "bad M/N/K"), (_gated, dict(dt=2), 1, "dtype"),
+    (_lbwd, dict(z=None), 1, "null"), (_lbwd, dict(dy=None), 1, "null"), (_lbwd, dict(ldy=31), 1, "stride"),
+    (_lbwd, dict(ldz=31), 1, "stride"), (_lbwd, dict(lddx=60), 1, "stride"), (_lbwd, dict(lddw=60), 1, "stride"),
+    (_lbwd, dict(ddt=3), 1, "db_dtype"), (_lbwd, dict(n=64), 4, "needs"), (_lbwd, dict(ws=P + 8), 4, "aligned"),
+    (_lbwd, dict(K=0), 1, "bad M/N/K"), (_lbwd, dict(dt=2), 1, "dtype"), (_lbwd, dict(act=9), 1, "act"),
+    (_lbwd, dict(dx=None, dw=None, db=None, ws=None, n=0), 0, ""),
+    (_lbwd, dict(M=0, dw=None, db=None, dy=None), 0, ""),
+    (_gbwd, dict(zg=None), 1, "null"), (_gbwd, dict(wg=None), 1, "null"), (_gbwd, dict(ldz=31), 1, "stride"),
+    (_gbwd, dict(lddw=60, dwg=None), 1, "stride"), (_gbwd, dict(ddt=-1, dbg=None), 1, "db_dtype"),
+    (_gbwd, dict(ws=None), 4, "needs"), (_gbwd, dict(dt=3), 1, "dtype"),
+    (_gbwd, dict(dx=None, dw=None, dwg=None, db=None, dbg=None, ws=None, n=0), 0, ""),
     (_norm, dict(M=-1), 1, "M must be"), (_norm, dict(D_=0), 1, "D 1"), (_norm, dict(D_=(1 << 24) + 1), 1, "2\\^24"),
     (_norm, dict(xdt=3), 1, "x_dtype"), (_norm, dict(w=P, wdt=3), 1, "w_dtype"), (_norm, dict(y=None), 1, "null"),
     (_norm, dict(ldx=7), 1, "stride"), (_norm, dict(M=0, x=None), 0, ""),
@@ -218,16 +226,31 @@ def test_c_abi_refusals(call, kw, code, match):
         assert re.search(match, msg), msg
 
 
-def test_c_abi_workspace_refusals():
+def test_c_abi_layer_norm_bwd():
     rc, msg = _rc("dc_layer_norm_bwd", P, 8, P, 8, 0, None, 0, P, None, 8, P, P, 4, 8, None, 0, None)
     assert rc == 4 and "workspace" in msg
-    rc, msg = _rc("dc_act16_bwd", P, 64, None, 0, 0, None, 0, P, 0, 0, 4, 64, P, 8, None)
-    assert rc == 4 and "workspace" in msg
-    rc, msg = _rc("dc_act16_bwd", P, 64, P, 64, 1, P, 56, None, -1, 0, 4, 64, None, 0, None)
-    assert rc == 2 and "rounded up to 64" in msg
-    rc, msg = _rc("dc_act16_bwd", P, 64, P, 64, 1, None, 64, None, -1, 0, 4, 64, None, 0, None)
-    assert rc == 1 and "together" in msg
-    rc, msg = _rc("dc_gated16_bwd", P, 64, P, None, 64, 1, P, P, 64, None, None, -1, 0, 4, 64, None, 0, None)
+    rc, msg = _rc("dc_layer_norm_bwd", P, 7, P, 8, 0, None, 0, P, P, 8, None, None, 4, 8, None, 0, None)
+    assert rc == 1 and "stride" in msg
+    rc, msg = _rc("dc_layer_norm_bwd", P, 8, P, 8, 0, None, 0, None, P, 8, None, None, 4, 8, None, 0, None)
     assert rc == 1 and "null" in msg
     assert _rc("dc_layer_norm_bwd", P, 8, P, 8, 0, None, 0, P, None, 8, None, None, 4, 8, None, 0, None)[0] == 0
-    assert ctypes.sizeof(ctypes.c_size_t) == 8
+
+
+def test_workspace_queries_cover_padded_operands():
+    """An operand that has to be copied adds its padded size; aligned ones of a
+    shape that is not split add nothing."""
+    so = _lib.lib()
+    if so is None:
+        pytest.skip("library not built")
+    M, N, K = 4096, 4096, 2048
+    q = so.dc_linear16_workspace_bytes
+    assert q(P, K, P, K, M, N, K) == 0
+    assert q(P + 2, K, P, K, M, N, K) == 2 * M * K
+    assert q(P, K + 1, P + 2, K, M, N, K) == 2 * (M + N) * K
+    assert q(P, K - 1, P, K - 1, M, N, K - 1) == 2 * (M + N) * K
+    g = so.dc_gated16_workspace_bytes
+    assert g(P, K, P, K, P + 2, K, M, N, K) == 2 * N * K
+    b = so.dc_linear16_bwd_workspace_bytes
+    assert b(P, N, P, K, P, K, 0, 1, M, N, K) == 0
+    assert b(P, N, P, K, P, K, 1, 1, M, N, K) == 2 * M * N   # dz
+    assert q(P, 0, P, 0, 0, N, K) == 0 and b(P, 0, P, 0, P, 0, 0, 15, M, N, 0) == 0
