@@ -18,9 +18,9 @@
 //   fragment (8 k of one row) is one 16-byte read.
 // RC stage: [64 k][rows]; a fragment is two ds_read_b64_tr_b16, each of which
 //   takes a 4 (k) x 16 (rows) block per 16 lanes and hands every lane the 4 k
-//   of its row. 16-row pair of chunks p of line k sits at p ^ (k & 3), bit 2
-//   flipped for odd p: the four lines of a block fall on different banks, and
-//   so do the two blocks of a 32-row fragment.
+//   of its row. 16-row pair of chunks p of line k sits at p ^ (k & 3), and in
+//   lines of whole 256 bytes with bit 2 flipped for odd p: the four lines of a
+//   block fall on different banks, and so do the two blocks of a 32-row fragment.
 //
 // The contraction's end inside a stage: loads clamp to the last k (rows to the
 // last row), and the last stage's fragments are masked.
@@ -98,12 +98,12 @@ __device__ __forceinline__ int2 lds_read_tr(const uint8_t* p) {
 template <int R>
 __device__ __forceinline__ int rc_physical(int p, int k) {
   const int q = p ^ (k & 3);
-  return R >= 128 ? q ^ ((p & 1) << 2) : q;
+  return R % 128 == 0 ? q ^ ((p & 1) << 2) : q;
 }
 template <int R>
 __device__ __forceinline__ int rc_logical(int q, int k) {
   const int p = q ^ (k & 3);
-  return R >= 128 ? p ^ ((p & 1) << 2) : p;
+  return R % 128 == 0 ? p ^ ((p & 1) << 2) : p;
 }
 
 // Keeps the `valid` (0 .. 8) first of a fragment's 8 values.
@@ -167,8 +167,9 @@ __device__ __forceinline__ void rows_pre(const v16f (&acc)[FN][FM], uint8_t* sta
         *reinterpret_cast<float4*>(stage + l32 * RP + 4 * (32 * i + 8 * g + 4 * hf)) =
             make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
     wave_lds_fence();
-#pragma unroll 1
-    for (int r = lane / CH; r < 32; r += 64 / CH) {
+#pragma unroll
+    for (int k = 0; k < 32 * CH / 64; ++k) {
+      const int r = lane / CH + k * (64 / CH);
       float v[8], g[8];
 #pragma unroll
       for (int q = 0; q < 8; q += 4) {
@@ -489,33 +490,35 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
       if constexpr (GATED) bg[e] = b_l[brow + 32 + e];
     }
     const int n = nb + 8 * oc;
-    rows_pre<FN, FM, GATED>(acc, share, lane, [&](int r, float (&v)[8], float (&g)[8]) __attribute__((always_inline)) {
-      const int m = mb + r;
-      if (m >= p.M || n >= p.N) return;
+    // one uniform branch around the whole of it, so that the steps of a block overlap
+    with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
+      constexpr int ACT = decltype(act_)::value;
+      if constexpr (GATED && ACT == DC_ACT_NONE) return;   // refused by the host
+      rows_pre<FN, FM, GATED>(acc, share, lane, [&](int r, float (&v)[8], float (&g)[8]) __attribute__((always_inline)) {
+        const int m = mb + r;
+        if (m >= p.M || n >= p.N) return;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] += bv[e];
-        if constexpr (GATED) g[e] += bg[e];
-      }
-      if (p.z) {
-        store8_n(p.z + (int64_t)m * p.ldz + n, p.N - n, v);
-        if constexpr (GATED) store8_n(p.z2 + (int64_t)m * p.ldz + n, p.N - n, g);
-      }
-      with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
-        constexpr int ACT = decltype(act_)::value;
+        for (int e = 0; e < 8; ++e) {
+          v[e] += bv[e];
+          if constexpr (GATED) g[e] += bg[e];
+        }
+        if (p.z) {
+          store8_n(p.z + (int64_t)m * p.ldz + n, p.N - n, v);
+          if constexpr (GATED) store8_n(p.z2 + (int64_t)m * p.ldz + n, p.N - n, g);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if constexpr (GATED) v[e] *= act_value<ACT>(g[e]);
           else v[e] = act_value<ACT>(v[e]);
         }
-      });
-      if (!GATED && p.res) {
-        float s[8];
-        load8_n<DT>(p.res + (int64_t)m * p.ldr + n, p.N - n, s);
+        if (!GATED && p.res) {
+          float s[8];
+          load8_n<DT>(p.res + (int64_t)m * p.ldr + n, p.N - n, s);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += s[e];
-      }
-      store_chunk16(p.out + (int64_t)m * p.ldo + n, p.N - n, pack8<DT>(v));
+          for (int e = 0; e < 8; ++e) v[e] += s[e];
+        }
+        store_chunk16(p.out + (int64_t)m * p.ldo + n, p.N - n, pack8<DT>(v));
+      });
     });
   } else {
     rows_h16<DT, FN, FM>(acc, share, lane, [&](int r, int c, uint4 v) __attribute__((always_inline)) {
@@ -607,17 +610,24 @@ int launch16(const char* who, Gemm16 p, const Plan16& plan, hipStream_t st) {
 }
 
 // Tiles (n x m); EPI_GATED ones hold half as many channels.
-typedef Tile16<4, 2, 2, 4, 2, 2> T256x256;    // 8 waves of 64 x 128, 128 KB
+typedef Tile16<4, 2, 2, 4, 2, 2> T256x256;    // 8 waves of 64 x 128, 128 KB: 1 per CU
+typedef Tile16<4, 2, 2, 3, 2, 2> T256x192;    // 8 waves of 64 x 96, 112 KB: 1 per CU
+typedef Tile16<4, 2, 2, 2, 3, 2> T256x128;    // 8 waves of 64 x 64, 144 KB: 1 per CU
+typedef Tile16<2, 4, 2, 2, 3, 2> T128x256;    // 8 waves of 64 x 64, 144 KB: 1 per CU
 typedef Tile16<2, 2, 2, 2, 2, 2> T128x128;    // 4 waves of 64 x 64, 64 KB: 2 per CU
 typedef Tile16<2, 4, 2, 1, 3, 2> T128x128d;   // 8 waves of 64 x 32, 96 KB: 1 per CU
 typedef Tile16<1, 4, 2, 1, 3, 2> T64x128;     // 4 waves of 64 x 32, 72 KB: 2 per CU
 typedef Tile16<1, 2, 2, 1, 3, 2> T64x64;      // 2 waves of 64 x 32, 48 KB: 3 per CU
-enum { TILE_256x256 = 0, TILE_128x128 = 1, TILE_128x128D = 2, TILE_64x128 = 3, TILE_64x64 = 4 };
+enum { TILE_256x256 = 0, TILE_128x128 = 1, TILE_128x128D = 2, TILE_64x128 = 3, TILE_64x64 = 4, TILE_256x192 = 5,
+       TILE_256x128 = 6, TILE_128x256 = 7 };
 
 template <int DT, bool A_RC, bool W_RC, int EPI>
 int run_tile16(const char* who, const Gemm16& p, const Plan16& plan, hipStream_t st) {
   switch (plan.tile) {
     case TILE_256x256: return launch16<T256x256, DT, A_RC, W_RC, EPI>(who, p, plan, st);
+    case TILE_256x192: return launch16<T256x192, DT, A_RC, W_RC, EPI>(who, p, plan, st);
+    case TILE_256x128: return launch16<T256x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);
+    case TILE_128x256: return launch16<T128x256, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_128x128: return launch16<T128x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_128x128D: return launch16<T128x128d, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_64x128: return launch16<T64x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);

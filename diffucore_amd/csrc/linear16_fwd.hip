@@ -29,23 +29,55 @@ int check_scratch(const char* who, size_t need, const void* ws, size_t ws_bytes)
   return DC_EWORKSPACE;
 }
 
+// Tile and k slices by the least of a fitted time, in us:
+//   T = fixed + h (round + stage * stages)  [+ 2.9 + 0.32 per MB of partial sums when k is split]
+// where a round fills every CU with `per` workgroups of the tile and h counts
+// rounds; a last round in which the busiest CU holds j < per of them counts
+// level[j - 1], and any level that is not full on every CU counts up to `slack`
+// less (the clock rises and memory frees as CUs fall idle). Fitted to 20000 random
+// products of 17 to 16384 rows, 16 to 20480 channels and 64 to 8192 of k (all
+// three operand layouts, 8 tiles, up to 16 slices; operands rotated through
+// memory): rms error of a time 9 to 13%, and the pick is 2.5% off the best of all
+// tiles and slices on average, 1.6% for products past 40 GFLOP. A rule that went
+// by the number of 128 x 128 tiles was 6.9% off. At 256 x 256 / 256 x 192 / 128 x
+// 128: 4608 x 2048 -> 8192 191 / 153 / 160 us, 8192 x 2560 -> 640 59 / 49 / 36,
+// dw of 4608 x (2048, 8192) 129 / 188 / 157.
+struct TileCost {
+  int tile, bn, bm, per;
+  float fixed, round, stage, slack, level[2];
+};
+static constexpr TileCost COSTS[] = {
+    {TILE_256x256, 256, 256, 1, 3.25f, 7.61f, 1.791f, 0.35f, {}},
+    {TILE_256x192, 256, 192, 1, 2.98f, 5.65f, 1.527f, 0.38f, {}},
+    {TILE_256x128, 256, 128, 1, 3.39f, 4.55f, 0.997f, 0.33f, {}},
+    {TILE_128x256, 128, 256, 1, 3.32f, 4.59f, 1.007f, 0.34f, {}},
+    {TILE_128x128, 128, 128, 2, 4.08f, 3.27f, 1.053f, 0.27f, {0.78f}},
+    {TILE_128x128D, 128, 128, 1, 4.49f, 2.77f, 0.570f, 0.32f, {}},
+    {TILE_64x128, 64, 128, 2, 5.89f, 1.64f, 0.710f, 0.22f, {0.53f}},
+    {TILE_64x64, 64, 64, 3, 6.25f, 1.36f, 0.691f, 0.12f, {0.40f, 0.60f}},
+};
+
 Plan16 plan16(int64_t M, int64_t rows, int64_t nk, int problems) {
   const int64_t cus = device_cus();
-  const auto tiles = [&](int bn, int bm) { return ((rows + bn - 1) / bn) * ((M + bm - 1) / bm) * problems; };
-  const int64_t t128 = tiles(128, 128);
-  Plan16 r{TILE_256x256, 1, (int)nk};
-  if (t128 <= cus / 2) r.tile = tiles(64, 128) < cus / 2 ? TILE_64x64 : TILE_64x128;
-  else if (t128 <= cus) r.tile = TILE_128x128D;
-  else if (t128 <= 2 * cus) r.tile = TILE_128x128;
-  if (t128 > cus / 2) return r;
-  const int64_t used = r.tile == TILE_64x64 ? tiles(64, 64) : tiles(64, 128);
-  int64_t s = 2 * cus / used;
-  if (s > nk / 8) s = nk / 8;
-  if (s > 16) s = 16;
-  if (s < 2) return r;
-  r.kstages = (int)((nk + s - 1) / s);
-  r.splits = (int)((nk + r.kstages - 1) / r.kstages);
-  return r;
+  const float mb = (float)((double)M * (double)rows * problems * 4e-6);
+  Plan16 best{TILE_256x256, 1, (int)nk};
+  float least = 1e30f;
+  for (const TileCost& c : COSTS) {
+    const int64_t tiles = (rows + c.bn - 1) / c.bn * ((M + c.bm - 1) / c.bm) * problems;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      // slices of 4 stages or more, of products that leave CUs idle
+      if (s > 1 && (tiles > cus || nk < 4 * s)) break;
+      const int64_t stages = (nk + s - 1) / s, splits = stages ? (nk + stages - 1) / stages : 1;
+      const int64_t units = tiles * splits, slots = cus * c.per;
+      const int64_t rest = units % slots, j = (rest + cus - 1) / cus;   // j: on the busiest CU of the last round
+      float h = (float)(units / slots);
+      if (j) h += (j < c.per ? c.level[j - 1] : 1.0f) * (1.0f - c.slack * (1.0f - (float)rest / (float)(cus * j)));
+      float t = c.fixed + h * (c.round + c.stage * (float)stages);
+      if (splits > 1) t += 2.9f + 0.32f * mb * (float)splits;
+      if (t < least) least = t, best = {c.tile, (int)splits, (int)stages};
+    }
+  }
+  return best;
 }
 
 // A forward call's scratch: copies of the operands that need one, split-K sums.
