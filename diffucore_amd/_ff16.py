@@ -12,7 +12,7 @@ runs torch's own ops there (``unet.py:148-183``).
 All of them take tensors of any leading shape and any strides, enqueue on
 torch's current stream of the tensors' device, and are differentiable once.
 Sums, statistics and gradients are accumulated in float32 and rounded once; for
-the backward pass of an activation its input is kept in float32, and the
+the backward pass of an activation its input is kept in 24 bits, and the
 gradient at it is rounded to 16 bits as the operand of the products that follow.
 CPU tensors run the same formulas in torch ops; GPU tensors always run the
 HIP kernels, and raise where the library is missing.
@@ -249,13 +249,13 @@ def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
         return out, None
     bias = _contig(bias)
     r2 = None if residual is None else _flat(residual)
-    z = torch.empty((M, N), device=dev, dtype=torch.float32) if keep else None
+    z = torch.empty(3 * M * N, device=dev, dtype=torch.uint8) if keep else None   # dc_saved16_bytes
     ldx, ldw = x2.stride(0), w2.stride(0)
     with _lib.device_ctx(dev):
         need = _scratch_bytes("dc_linear16_workspace_bytes", dev.index, _at(x2), ldx, _at(w2), ldw, M, N, K)
         ws = _scratch(need, dev)
         rc = so.dc_linear16(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(bias), _code(bias), _ptr(r2),
-                            0 if r2 is None else r2.stride(0), act, out.data_ptr(), N, _ptr(z), N, dt, M, N, K,
+                            0 if r2 is None else r2.stride(0), act, out.data_ptr(), N, _ptr(z), dt, M, N, K,
                             _ptr(ws), need, _lib.stream_ptr(dev))
     _lib.check(rc, "dc_linear16")
     return out, z
@@ -293,7 +293,7 @@ class _LinearAct(torch.autograd.Function):
             need = _scratch_bytes("dc_linear16_bwd_workspace_bytes", dev.index, _at(dy2), ldy, _at(x2), ldx, _at(w2),
                                   ldw, ctx.act, want, M, N, K)
             ws = _scratch(need, dev)
-            rc = so.dc_linear16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), N, ctx.act,
+            rc = so.dc_linear16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), ctx.act,
                                     _ptr(dx), K, _ptr(dw), K, _ptr(db), _code(db), _lib.dtype_code(dt), M, N, K,
                                     _ptr(ws), need, _lib.stream_ptr(dev))
         _lib.check(rc, "dc_linear16_bwd")
@@ -362,7 +362,8 @@ def _gated_forward(x, weight, bias, gate_weight, gate_bias, act: int, keep: bool
     bv, bg = _ptr(bias), _ptr(gate_bias)
     if gate_weight is None and bias is not None:
         bg = bv + N * bias.element_size()
-    z = torch.empty((2, M, N), device=dev, dtype=torch.float32) if keep else None
+    half = -(-3 * M * N // 16) * 16   # dc_saved16_bytes, the next one aligned
+    z = torch.empty(2 * half, device=dev, dtype=torch.uint8) if keep else None
     zv = _ptr(z)
     ldx, ldv, ldg = x2.stride(0), wv.stride(0), wg.stride(0)
     with _lib.device_ctx(dev):
@@ -371,7 +372,7 @@ def _gated_forward(x, weight, bias, gate_weight, gate_bias, act: int, keep: bool
         ws = _scratch(need, dev)
         rc = so.dc_gated16(x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, bv, bg,
                            _code(bias if bias is not None else gate_bias), act, out.data_ptr(), N, zv,
-                           None if z is None else zv + M * N * 4, N, _lib.dtype_code(x.dtype), M, N, K, _ptr(ws), need,
+                           None if z is None else zv + half, _lib.dtype_code(x.dtype), M, N, K, _ptr(ws), need,
                            _lib.stream_ptr(dev))
     _lib.check(rc, "dc_gated16")
     return out, z
@@ -418,7 +419,7 @@ class _GatedLinear(torch.autograd.Function):
                                   _at(wg), ldg, want, M, N, K)
             ws = _scratch(need, dev)
             rc = so.dc_gated16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, zv,
-                                   zv + M * N * 4, N, ctx.act, _ptr(dx), K, dwv_p, dwg_p, K, dbv_p, dbg_p,
+                                   zv + z.numel() // 2, ctx.act, _ptr(dx), K, dwv_p, dwg_p, K, dbv_p, dbg_p,
                                    _lib.NONE if ctx.bias_dtype is None else _lib.dtype_code(ctx.bias_dtype),
                                    _lib.dtype_code(dt), M, N, K, _ptr(ws), need, _lib.stream_ptr(dev))
         _lib.check(rc, "dc_gated16_bwd")

@@ -57,15 +57,16 @@ _SIGS = {
                                       ctypes.POINTER(_I64), ctypes.c_float, _P]),
     "dc_int8_attn_quantize_q": (_I, [_P, _I, _I, _I, _I, _I, ctypes.POINTER(_I64), _P, _P, _P]),
     "dc_linear16_workspace_bytes": (_Z, [_P, _I64, _P, _I64, _I64, _I64, _I64]),
-    "dc_linear16": (_I, [_P, _I64, _P, _I64, _P, _I, _P, _I64, _I, _P, _I64, _P, _I64, _I, _I64, _I64, _I64, _P, _Z, _P]),
+    "dc_saved16_bytes": (_Z, [_I64, _I64]),
+    "dc_linear16": (_I, [_P, _I64, _P, _I64, _P, _I, _P, _I64, _I, _P, _I64, _P, _I, _I64, _I64, _I64, _P, _Z, _P]),
     "dc_gated16_workspace_bytes": (_Z, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64]),
-    "dc_gated16": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64,
-                        _P, _Z, _P]),
+    "dc_gated16": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _I, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _P,
+                        _Z, _P]),
     "dc_linear16_bwd_workspace_bytes": (_Z, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I64, _I64, _I64]),
-    "dc_linear16_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _I, _I, _I64, _I64,
+    "dc_linear16_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _I64, _P, _I64, _P, _I, _I, _I64, _I64,
                              _I64, _P, _Z, _P]),
     "dc_gated16_bwd_workspace_bytes": (_Z, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I64, _I64, _I64]),
-    "dc_gated16_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _P, _I64, _P, _P, _I64, _P, _P,
+    "dc_gated16_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I, _P, _I64, _P, _P, _I64, _P, _P,
                             _I, _I, _I64, _I64, _I64, _P, _Z, _P]),
     "dc_layer_norm": (_I, [_P, _I64, _I, _P, _P, _I, ctypes.c_float, _P, _I64, _P, _I64, _I64, _P]),
     "dc_layer_norm_bwd_workspace_bytes": (_Z, [_I64, _I64, _I]),

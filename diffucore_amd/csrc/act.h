@@ -168,6 +168,33 @@ __device__ __forceinline__ void store_chunk16(uint16_t* p, int64_t n, uint4 v) {
   if (k & 2) store_words<uint16_t, 1>(p + (k & 4), {{bc}});
   if (k & 1) p[k & 6] = (uint16_t)(k & 2 ? cz : bc);
 }
+// 8 bytes of a row of which `n` are left.
+__device__ __forceinline__ uint2 load_chunk8(const uint8_t* p, int64_t n) {
+  if (n >= 8) {
+    const auto u = load_words<uint8_t, 2>(p);
+    return make_uint2(u.v[0], u.v[1]);
+  }
+  const int k = n > 0 ? (int)n : 0;
+  uint32_t a = 0u, t = 0u;   // the first four, and what follows them
+  if (k & 4) a = load_words<uint8_t, 1>(p).v[0];
+  const uint8_t* q = p + (k & 4);
+  for (int e = 0; e < (k & 3); ++e) t |= (uint32_t)q[e] << (8 * e);
+  return k & 4 ? make_uint2(a, t) : make_uint2(t, 0u);
+}
+__device__ __forceinline__ void store_chunk8(uint8_t* p, int64_t n, uint2 v) {
+  if (n >= 8) {
+    store_words<uint8_t, 2>(p, {{v.x, v.y}});
+    return;
+  }
+  const int k = n > 0 ? (int)n : 0;
+  uint32_t t = v.x;
+  if (k & 4) {
+    store_words<uint8_t, 1>(p, {{v.x}});
+    t = v.y;
+  }
+  uint8_t* q = p + (k & 4);
+  for (int e = 0; e < (k & 3); ++e) q[e] = (uint8_t)(t >> (8 * e));
+}
 __device__ __forceinline__ float4 load_chunk32(const float* p, int64_t n) {
   float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
   if (n >= 4) {

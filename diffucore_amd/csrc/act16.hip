@@ -3,14 +3,14 @@
 // two products that follow, with the bias gradients' column sums taken from
 // the float32 values on the way.
 //
-//   linear  dz = dy act'(z)                          reads 2 + 4 bytes an element, writes 2
-//   gated   dzv = dy act(zg), dzg = dy zv act'(zg)   reads 2 + 8, writes 4
+//   linear  dz = dy act'(z)                          reads 2 + 3 bytes an element, writes 2
+//   gated   dzv = dy act(zg), dzg = dy zv act'(zg)   reads 2 + 6, writes 4
 //   sums    db = sum over rows of dy                 reads 2
 //
-// The pre-activations z are float32: rounded to 16 bits they cost a third
+// The pre-activations z are kept in 24 bits. Rounded to 16 they cost a third
 // rounding of the same size as dz's own and the result's (bf16 gated gradients
 // 0.0031 off in relative L2 where the rounding of the result alone is 0.0017,
-// 0.0024 with float32).
+// 0.0024 with 24 bits or 32).
 //
 // Memory-bound: one pass, 16 bytes a lane and access. A workgroup takes 8 * TX
 // columns (TX lanes of 8 columns) and every TYth row of a block of rows, sums
@@ -22,12 +22,12 @@ namespace dc {
 
 struct ActBwdArgs {
   const uint16_t* dy;
-  const float* za;      // linear: z; gated: the value's pre-activation
-  const float* zg;
+  const uint8_t* za;    // linear: z; gated: the value's pre-activation (store_saved8)
+  const uint8_t* zg;
   uint16_t* da;         // linear: dz; gated: the value's gradient
   uint16_t* dg;
   float* part;          // [P][1 or 2][N], NULL: no sums
-  int64_t lddy, ldz, lddz;
+  int64_t lddy, lddz;
   int M, N, pad;        // pad: columns of dz to fill (its row stride)
   int tx_log, rows;     // log2 TX; rows per workgroup
   int act;
@@ -46,8 +46,8 @@ __device__ __forceinline__ void act_bwd_rows(const ActBwdArgs& p, int64_t col, i
 #pragma unroll
       for (int e = 0; e < 8; ++e) sa[e] += dy[e];
     } else {
-      load8_n(p.za + r * p.ldz + col, n, a);
-      if constexpr (MODE == 2) load8_n(p.zg + r * p.ldz + col, n, g);
+      load_saved8(p.za, p.M, p.N, r, col, a);
+      if constexpr (MODE == 2) load_saved8(p.zg, p.M, p.N, r, col, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float value;
@@ -175,7 +175,7 @@ static int run_act_bwd(const char* who, ActBwdArgs p, int dtype, void* db0, void
 int act16_bwd(const char* who, const ActBwd& a, hipStream_t st) {
   ActBwdArgs p{};
   p.dy = static_cast<const uint16_t*>(a.dy), p.lddy = a.lddy, p.M = (int)a.M, p.N = (int)a.N;
-  p.za = a.zv, p.zg = a.zg, p.ldz = a.ldz, p.act = a.act;
+  p.za = a.zv, p.zg = a.zg, p.act = a.act;
   p.da = static_cast<uint16_t*>(a.dzv), p.dg = static_cast<uint16_t*>(a.dzg), p.lddz = a.lddz, p.pad = (int)a.lddz;
   p.part = a.dbv || a.dbg ? a.part : nullptr;
   if (a.zg) return run_act_bwd<2>(who, p, a.dtype, a.dbv, a.dbg, a.db_dtype, st);

@@ -18,8 +18,7 @@ int reduce_partials(const float* part, int P, int sections, int64_t width, void*
 struct ActBwd {
   const void* dy;
   int64_t lddy;
-  const float *zv, *zg;
-  int64_t ldz;
+  const uint8_t *zv, *zg;   // saved (saved16_bytes each)
   int act;
   void *dzv, *dzg;
   int64_t lddz;
@@ -70,6 +69,44 @@ __device__ __forceinline__ void load8_n(const float* p, int64_t n, float (&f)[8]
 __device__ __forceinline__ void store8_n(float* p, int64_t n, const float (&f)[8]) {
   store_chunk32(p, n, make_float4(f[0], f[1], f[2], f[3]));
   store_chunk32(p + 4, n - 4, make_float4(f[4], f[5], f[6], f[7]));
+}
+
+// Pre-activations kept for the backward pass: the upper 24 bits of a float32
+// (16 significant bits, off by at most 2^-16 of the value, inf and NaN as they
+// are), as a plane of 16-bit halves [M, N] and then a plane of bytes [M, N].
+// float32 would cost a third more of what bounds these passes (gated 4096 x 1280
+// -> 5120 with gradients: see act16.hip), bf16 or fp16 a rounding as large as
+// the result's own.
+inline size_t saved16_bytes(int64_t M, int64_t N) { return 3 * (size_t)M * (size_t)N; }
+
+__device__ __forceinline__ void store_saved8(uint8_t* z, int64_t M, int64_t N, int64_t m, int64_t n,
+                                             const float (&f)[8]) {
+  uint32_t h[4], l[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __float_as_uint(f[2 * i]), b = __float_as_uint(f[2 * i + 1]);
+    h[i] = __builtin_amdgcn_perm(b, a, 0x07060302);   // the upper halves of a and b
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i]), 0x0c0c0501);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(f[4 * i + 3]), __float_as_uint(f[4 * i + 2]), 0x0c0c0501);
+    l[i] = ab | cd << 16;                             // byte 1 of each
+  }
+  store_chunk16(reinterpret_cast<uint16_t*>(z) + m * N + n, N - n, make_uint4(h[0], h[1], h[2], h[3]));
+  store_chunk8(z + 2 * M * N + m * N + n, N - n, make_uint2(l[0], l[1]));
+}
+__device__ __forceinline__ void load_saved8(const uint8_t* z, int64_t M, int64_t N, int64_t m, int64_t n,
+                                            float (&f)[8]) {
+  const uint4 u = load_chunk16(reinterpret_cast<const uint16_t*>(z) + m * N + n, N - n);
+  const uint2 v = load_chunk8(z + 2 * M * N + m * N + n, N - n);
+  const uint32_t h[4] = {u.x, u.y, u.z, u.w}, l[2] = {v.x, v.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = l[i / 2] >> (16 * (i % 2));
+    f[2 * i] = __uint_as_float(h[i] << 16 | (b & 0xffu) << 8);
+    f[2 * i + 1] = __uint_as_float((h[i] & 0xffff0000u) | (b & 0xff00u));
+  }
 }
 
 }  // namespace dc

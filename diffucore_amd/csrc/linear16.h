@@ -45,8 +45,8 @@ struct Gemm16 {
   const void *bias, *bias2;
   const uint16_t* res;
   uint16_t *out, *out2;
-  float *z, *z2;
-  int64_t ldr, ldo, ldz;
+  uint8_t *z, *z2;          // store_saved8
+  int64_t ldr, ldo;
   // split-K: blockIdx.y takes `kstages` stages and writes float32 sums to
   // part + (y * problems + problem) * M * width, row stride `width`
   float* part;
@@ -503,8 +503,8 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
           if constexpr (GATED) g[e] += bg[e];
         }
         if (p.z) {
-          store8_n(p.z + (int64_t)m * p.ldz + n, p.N - n, v);
-          if constexpr (GATED) store8_n(p.z2 + (int64_t)m * p.ldz + n, p.N - n, g);
+          store_saved8(p.z, p.M, p.N, m, n, v);
+          if constexpr (GATED) store_saved8(p.z2, p.M, p.N, m, n, g);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -564,8 +564,8 @@ __global__ void __launch_bounds__(256) linear16_join_kernel(Gemm16 p) {
       if constexpr (GATED) g[e] += bias_at(p.bias2, p.bias_dtype, n + e);
     }
     if (p.z) {
-      store8_n(p.z + m * p.ldz + n, left, v);
-      if constexpr (GATED) store8_n(p.z2 + m * p.ldz + n, left, g);
+      store_saved8(p.z, p.M, p.N, m, n, v);
+      if constexpr (GATED) store_saved8(p.z2, p.M, p.N, m, n, g);
     }
     with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
       constexpr int ACT = decltype(act_)::value;

@@ -101,7 +101,7 @@ extern "C" size_t dc_linear16_bwd_workspace_bytes(const void* dy, int64_t lddy, 
 }
 
 extern "C" int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                               const float* z, int64_t ldz, int act, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                               const void* z, int act, void* dx, int64_t lddx, void* dw, int64_t lddw,
                                void* db, int db_dtype, int dtype, int64_t M, int64_t N, int64_t K, void* ws,
                                size_t ws_bytes, void* stream) {
   clear_error();
@@ -120,12 +120,12 @@ extern "C" int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int6
   if (!dx && !dw && !db) return DC_OK;
   const bool act_z = act != DC_ACT_NONE;
   if (!dy || !x || !w || (act_z && !z)) return refuse(DC_EINVAL, who, "null pointer");
-  if (lddy < N || ldx < K || ldw < K || (act_z && ldz < N))
+  if (lddy < N || ldx < K || ldw < K)
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const Backward16 b({dy, lddy, M, N}, {x, ldx, M, K}, {w, ldw, N, K}, {}, act_z, dx, dw ? 1 : 0, db, ws);
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
   if (act_z || db) {
-    const ActBwd a{dy, lddy, act_z ? z : nullptr, nullptr, ldz, act, const_cast<void*>(act_z ? b.dz.p : nullptr),
+    const ActBwd a{dy, lddy, static_cast<const uint8_t*>(act_z ? z : nullptr), nullptr, act, const_cast<void*>(act_z ? b.dz.p : nullptr),
                    nullptr, round_up(N, 64), db, nullptr, db_dtype, dtype, M, N, b.part};
     if (int e = act16_bwd(who, a, st)) return e;
   }
@@ -147,7 +147,7 @@ extern "C" size_t dc_gated16_bwd_workspace_bytes(const void* dy, int64_t lddy, c
 }
 
 extern "C" int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* wv, int64_t ldwv,
-                              const void* wg, int64_t ldwg, const float* zv, const float* zg, int64_t ldz, int act,
+                              const void* wg, int64_t ldwg, const void* zv, const void* zg, int act,
                               void* dx, int64_t lddx, void* dwv, void* dwg, int64_t lddw, void* dbv, void* dbg,
                               int db_dtype, int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes,
                               void* stream) {
@@ -168,13 +168,13 @@ extern "C" int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64
   }
   if (!dx && !dwv && !dwg && !dbv && !dbg) return DC_OK;
   if (!dy || !x || !wv || !wg || !zv || !zg) return refuse(DC_EINVAL, who, "null pointer");
-  if (lddy < N || ldx < K || ldwv < K || ldwg < K || ldz < N)
+  if (lddy < N || ldx < K || ldwv < K || ldwg < K)
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const int dws = (dwv ? 1 : 0) + (dwg ? 1 : 0);
   const Backward16 b({dy, lddy, M, N}, {x, ldx, M, K}, {wv, ldwv, N, K}, {wg, ldwg, N, K}, true, dx, dws, dbv || dbg,
                      ws);
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
-  const ActBwd a{dy, lddy, zv, zg, ldz, act, const_cast<void*>(b.dz.p), const_cast<void*>(b.dzg.p), b.dz.ld, dbv, dbg,
+  const ActBwd a{dy, lddy, static_cast<const uint8_t*>(zv), static_cast<const uint8_t*>(zg), act, const_cast<void*>(b.dz.p), const_cast<void*>(b.dzg.p), b.dz.ld, dbv, dbg,
                  db_dtype, dtype, M, N, b.part};
   if (int e = act16_bwd(who, a, st)) return e;
   if (dx)

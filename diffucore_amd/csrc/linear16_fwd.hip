@@ -116,6 +116,8 @@ struct Forward16 {
 
 using namespace dc;
 
+extern "C" size_t dc_saved16_bytes(int64_t M, int64_t N) { return M > 0 && N > 0 ? saved16_bytes(M, N) : 0; }
+
 extern "C" size_t dc_linear16_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                               int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || check_product("dc_linear16", DC_F16, DC_ACT_NONE, M, N, K)) return 0;
@@ -123,15 +125,15 @@ extern "C" size_t dc_linear16_workspace_bytes(const void* x, int64_t ldx, const 
 }
 
 extern "C" int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
-                           const void* res, int64_t ldr, int act, void* out, int64_t ldo, float* z, int64_t ldz,
-                           int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream) {
+                           const void* res, int64_t ldr, int act, void* out, int64_t ldo, void* z, int dtype,
+                           int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream) {
   clear_error();
   const char* who = "dc_linear16";
   if (int e = check_product(who, dtype, act, M, N, K)) return e;
   if (M == 0 || N == 0) return DC_OK;
   if (!x || !w || !out) return refuse(DC_EINVAL, who, "null pointer");
   if (bias && !float_dtype(bias_dtype)) return refuse(DC_EINVAL, who, "bad bias_dtype");
-  if (ldx < K || ldw < K || ldo < N || (res && ldr < N) || (z && ldz < N))
+  if (ldx < K || ldw < K || ldo < N || (res && ldr < N))
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const Forward16 f({x, ldx, M, K}, {w, ldw, N, K}, {}, M, N, K, ws);
   if (int e = check_scratch(who, f.bytes, ws, ws_bytes)) return e;
@@ -139,7 +141,7 @@ extern "C" int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ld
   if (int e = f.pad(who, st)) return e;
   Gemm16 p = f.args(M, N, K);
   p.bias = bias, p.bias_dtype = bias_dtype, p.act = act, p.res = static_cast<const uint16_t*>(res), p.ldr = ldr;
-  p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = z, p.ldz = ldz;
+  p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = static_cast<uint8_t*>(z);
   return dtype == DC_BF16 ? run_tile16<DC_BF16, false, false, EPI_LINEAR>(who, p, f.plan, st)
                           : run_tile16<DC_F16, false, false, EPI_LINEAR>(who, p, f.plan, st);
 }
@@ -151,8 +153,8 @@ extern "C" size_t dc_gated16_workspace_bytes(const void* x, int64_t ldx, const v
 }
 
 extern "C" int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg, int64_t ldwg,
-                          const void* bv, const void* bg, int bias_dtype, int act, void* out, int64_t ldo, float* zv,
-                          float* zg, int64_t ldz, int dtype, int64_t M, int64_t N, int64_t K, void* ws,
+                          const void* bv, const void* bg, int bias_dtype, int act, void* out, int64_t ldo, void* zv,
+                          void* zg, int dtype, int64_t M, int64_t N, int64_t K, void* ws,
                           size_t ws_bytes, void* stream) {
   clear_error();
   const char* who = "dc_gated16";
@@ -161,7 +163,7 @@ extern "C" int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ld
   if (!x || !wv || !wg || !out) return refuse(DC_EINVAL, who, "null pointer");
   if ((bv || bg) && !float_dtype(bias_dtype)) return refuse(DC_EINVAL, who, "bad bias_dtype");
   if (!zv != !zg) return refuse(DC_EINVAL, who, "zv and zg go together");
-  if (ldx < K || ldwv < K || ldwg < K || ldo < N || (zv && ldz < N))
+  if (ldx < K || ldwv < K || ldwg < K || ldo < N)
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const Forward16 f({x, ldx, M, K}, {wv, ldwv, N, K}, {wg, ldwg, N, K}, M, N, K, ws);
   if (int e = check_scratch(who, f.bytes, ws, ws_bytes)) return e;
@@ -169,7 +171,7 @@ extern "C" int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ld
   if (int e = f.pad(who, st)) return e;
   Gemm16 p = f.args(M, N, K);
   p.bias = bv, p.bias2 = bg, p.bias_dtype = bias_dtype, p.act = act;
-  p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = zv, p.z2 = zg, p.ldz = ldz;
+  p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = static_cast<uint8_t*>(zv), p.z2 = static_cast<uint8_t*>(zg);
   return dtype == DC_BF16 ? run_tile16<DC_BF16, false, false, EPI_GATED>(who, p, f.plan, st)
                           : run_tile16<DC_F16, false, false, EPI_GATED>(who, p, f.plan, st);
 }

@@ -399,25 +399,27 @@ int dc_int8_attn_quantize_q(const void* q, int dtype, int B, int H, int Lq, int 
 /*
  * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once. bias [N] of
  * bias_dtype (DC_NONE: none), res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
- * GELU_TANH / SILU / QUICK_GELU. z (or NULL) takes the pre-activation
- * x w^T + bias for dc_linear16_bwd, in float32.
+ * GELU_TANH / SILU / QUICK_GELU. z (or NULL; 2-byte aligned,
+ * dc_saved16_bytes) takes the pre-activation x w^T + bias for dc_linear16_bwd:
+ * the upper 24 bits of its float32 values, a plane of halves and one of bytes.
  */
+size_t dc_saved16_bytes(int64_t M, int64_t N);
 size_t dc_linear16_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N,
                                    int64_t K);
 int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
-                const void* res, int64_t ldr, int act, void* out, int64_t ldo, float* z, int64_t ldz, int dtype,
+                const void* res, int64_t ldr, int act, void* out, int64_t ldo, void* z, int dtype,
                 int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * out[M, N] = (x wv^T + bv) * act(x wg^T + bg), both weights [N, K] (the two
  * halves of a GEGLU projection, or matrices of their own), rounded once; zv and
- * zg (both or neither NULL; one row stride) take the two pre-activations.
+ * zg (both or neither NULL) take the two pre-activations, as z above.
  */
 size_t dc_gated16_workspace_bytes(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg,
                                   int64_t ldwg, int64_t M, int64_t N, int64_t K);
 int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ldwv, const void* wg, int64_t ldwg, const void* bv,
-               const void* bg, int bias_dtype, int act, void* out, int64_t ldo, float* zv, float* zg, int64_t ldz,
-               int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
+               const void* bg, int bias_dtype, int act, void* out, int64_t ldo, void* zv, void* zg, int dtype,
+               int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 
 /*
  * Gradients of dc_linear16 and dc_gated16, each output NULL where it is not
@@ -432,13 +434,13 @@ enum { DC_WANT_DX = 1, DC_WANT_DW = 2, DC_WANT_DW2 = 4, DC_WANT_DB = 8 };
 size_t dc_linear16_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w,
                                        int64_t ldw, int act, int want, int64_t M, int64_t N, int64_t K);
 int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                    const float* z, int64_t ldz, int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
+                    const void* z, int act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db,
                     int db_dtype, int dtype, int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 size_t dc_gated16_bwd_workspace_bytes(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* wv,
                                       int64_t ldwv, const void* wg, int64_t ldwg, int want, int64_t M, int64_t N,
                                       int64_t K);
 int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* wv, int64_t ldwv,
-                   const void* wg, int64_t ldwg, const float* zv, const float* zg, int64_t ldz, int act, void* dx,
+                   const void* wg, int64_t ldwg, const void* zv, const void* zg, int act, void* dx,
                    int64_t lddx, void* dwv, void* dwg, int64_t lddw, void* dbv, void* dbg, int db_dtype, int dtype,
                    int64_t M, int64_t N, int64_t K, void* ws, size_t ws_bytes, void* stream);
 

@@ -6,10 +6,10 @@ most ``u |y|`` (``u`` half a step of its type, plus half the smallest
 subnormal) and by the float32 sum's error, ``(n + 16) 2^-23`` times the sum of
 the terms' magnitudes for ``n`` terms (twice the textbook ``n 2^-24``: matrix
 cores add in groups, and an activation adds a few ulp of its own). The backward
-passes of an activation start from its float32 input: the sum's error moves a
-slope by at most ``max|act''|`` (below 1.2 for every activation here) times
-itself and a value by ``max|act'|`` (below 1.2), and the products' operand
-``dz`` is rounded to 16 bits once.
+passes of an activation start from its input cut to 24 bits (``2^-16`` of it):
+that and the sum's error move a slope by at most ``max|act''|`` (below 1.2 for
+every activation here) times themselves and a value by ``max|act'|`` (below
+1.2), and the products' operand ``dz`` is rounded to 16 bits once.
 """
 
 from __future__ import annotations
@@ -20,6 +20,7 @@ import torch
 
 U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
 TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -127}
+CUT = 2.0 ** -16   # of a pre-activation kept for the backward pass
 BEND = 1.2   # bounds |act'| and |act''| of every activation
 
 
@@ -65,7 +66,7 @@ def linear(x, w, b, name, res, dt, dy=None, bias_dt=None):
         dz = dy * slope
         edz32 = 2.0 ** -20 * dz.abs()
         if name != "none":
-            edz32 = edz32 + dy.abs() * BEND * ez
+            edz32 = edz32 + dy.abs() * BEND * (ez + CUT * z.abs())
         edz = edz32 + (_round(dz, dt) if name != "none" else 0)
         out.update(_grads(x, [w], [dz], [edz], [edz32], dt, bias_dt or dt))
         out["dres"] = (dy, torch.zeros_like(dy))
@@ -101,7 +102,7 @@ def gated(x, wv, wg, bv, bg, name, dt, dy=None, bias_dt=None):
     out = {"y": (y, _round(y, dt) + ev * a.abs() + BEND * eg * v.abs() + BEND * ev * eg + 2.0 ** -20 * y.abs())}
     if dy is not None:
         dv, dg = dy * a, dy * v * slope
-        rv, rg = ev, eg
+        rv, rg = ev + CUT * v.abs(), eg + CUT * g.abs()
         ev32 = 2.0 ** -20 * dv.abs() + dy.abs() * BEND * rg
         eg32 = 2.0 ** -20 * dg.abs() + dy.abs() * (rv * slope.abs() + (v.abs() + rv) * BEND * rg)
         out.update(_grads(x, [wv, wg], [dv, dg], [ev32 + _round(dv, dt), eg32 + _round(dg, dt)], [ev32, eg32], dt,

@@ -164,25 +164,25 @@ def _rc(name, *args):
     return rc, so.dc_last_error().decode()
 
 
-def _linear(x=P, ldx=64, w=P, ldw=64, bias=None, bdt=-1, res=None, ldr=0, act=0, out=P, ldo=32, z=None, ldz=0, dt=1,
-            M=4, N=32, K=64, ws=None, n=0):
-    return _rc("dc_linear16", x, ldx, w, ldw, bias, bdt, res, ldr, act, out, ldo, z, ldz, dt, M, N, K, ws, n, None)
+def _linear(x=P, ldx=64, w=P, ldw=64, bias=None, bdt=-1, res=None, ldr=0, act=0, out=P, ldo=32, z=None, dt=1, M=4,
+            N=32, K=64, ws=None, n=0):
+    return _rc("dc_linear16", x, ldx, w, ldw, bias, bdt, res, ldr, act, out, ldo, z, dt, M, N, K, ws, n, None)
 
 
-def _gated(x=P, ldx=64, wv=P, wg=P, ldw=64, bv=None, bg=None, bdt=-1, act=1, out=P, ldo=32, zv=None, zg=None, ldz=0,
+def _gated(x=P, ldx=64, wv=P, wg=P, ldw=64, bv=None, bg=None, bdt=-1, act=1, out=P, ldo=32, zv=None, zg=None,
            dt=0, M=4, N=32, K=64, ws=None, n=0):
-    return _rc("dc_gated16", x, ldx, wv, ldw, wg, ldw, bv, bg, bdt, act, out, ldo, zv, zg, ldz, dt, M, N, K, ws, n, None)
+    return _rc("dc_gated16", x, ldx, wv, ldw, wg, ldw, bv, bg, bdt, act, out, ldo, zv, zg, dt, M, N, K, ws, n, None)
 
 
-def _lbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, z=P, ldz=32, act=1, dx=P, lddx=64, dw=P, lddw=64, db=P, ddt=0, dt=1,
+def _lbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, z=P, act=1, dx=P, lddx=64, dw=P, lddw=64, db=P, ddt=0, dt=1,
           M=4, N=32, K=64, ws=P, n=1 << 30):
-    return _rc("dc_linear16_bwd", dy, ldy, x, ldx, w, ldw, z, ldz, act, dx, lddx, dw, lddw, db, ddt, dt, M, N, K, ws, n,
+    return _rc("dc_linear16_bwd", dy, ldy, x, ldx, w, ldw, z, act, dx, lddx, dw, lddw, db, ddt, dt, M, N, K, ws, n,
                None)
 
 
-def _gbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, wg=P, zv=P, zg=P, ldz=32, act=1, dx=P, lddx=64, dw=P, dwg=P, lddw=64,
+def _gbwd(dy=P, ldy=32, x=P, ldx=64, w=P, ldw=64, wg=P, zv=P, zg=P, act=1, dx=P, lddx=64, dw=P, dwg=P, lddw=64,
           db=P, dbg=P, ddt=0, dt=1, M=4, N=32, K=64, ws=P, n=1 << 30):
-    return _rc("dc_gated16_bwd", dy, ldy, x, ldx, w, ldw, wg, ldw, zv, zg, ldz, act, dx, lddx, dw, dwg, lddw, db, dbg,
+    return _rc("dc_gated16_bwd", dy, ldy, x, ldx, w, ldw, wg, ldw, zv, zg, act, dx, lddx, dw, dwg, lddw, db, dbg,
                ddt, dt, M, N, K, ws, n, None)
 
 
@@ -196,21 +196,21 @@ def _norm(x=P, ldx=8, xdt=0, w=None, b=None, wdt=-1, y=P, ldy=8, stats=None, M=4
     (_linear, dict(dt=2), 1, "dtype"), (_linear, dict(act=3), 1, "act"), (_linear, dict(K=0), 1, "bad M/N/K"),
     (_linear, dict(x=None), 1, "null"), (_linear, dict(out=None), 1, "null"),
     (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"), (_linear, dict(ldo=31), 1, "stride"),
-    (_linear, dict(res=P, ldr=8), 1, "stride"), (_linear, dict(z=P, ldz=8), 1, "stride"),
+    (_linear, dict(res=P, ldr=8), 1, "stride"), 
     (_linear, dict(ldx=63), 1, "stride"), (_linear, dict(ldw=56), 1, "stride"),
     (_linear, dict(K=60, ldx=60, ldw=60), 4, "needs"), (_linear, dict(ldx=68), 4, "needs"),
     (_linear, dict(x=P + 8), 4, "needs"), (_linear, dict(x=P + 8, ws=P + 8, n=1 << 20), 4, "aligned"),
     (_linear, dict(M=0, x=None), 0, ""), (_linear, dict(N=0), 0, ""),
-    (_gated, dict(wg=None), 1, "null"), (_gated, dict(act=3), 1, "act"), (_gated, dict(zv=P, ldz=32), 1, "together"),
+    (_gated, dict(wg=None), 1, "null"), (_gated, dict(act=3), 1, "act"), (_gated, dict(zv=P), 1, "together"),
     (_gated, dict(bg=P, bdt=-1), 1, "bias_dtype"), (_gated, dict(wg=P + 2), 4, "needs"),
     (_gated, dict(M=0), 0, ""), (_gated, dict(K=0), 1, "bad M/N/K"), (_gated, dict(dt=2), 1, "dtype"),
     (_lbwd, dict(z=None), 1, "null"), (_lbwd, dict(dy=None), 1, "null"), (_lbwd, dict(ldy=31), 1, "stride"),
-    (_lbwd, dict(ldz=31), 1, "stride"), (_lbwd, dict(lddx=60), 1, "stride"), (_lbwd, dict(lddw=60), 1, "stride"),
+    (_lbwd, dict(lddx=60), 1, "stride"), (_lbwd, dict(lddw=60), 1, "stride"),
     (_lbwd, dict(ddt=3), 1, "db_dtype"), (_lbwd, dict(n=64), 4, "needs"), (_lbwd, dict(ws=P + 8), 4, "aligned"),
     (_lbwd, dict(K=0), 1, "bad M/N/K"), (_lbwd, dict(dt=2), 1, "dtype"), (_lbwd, dict(act=9), 1, "act"),
     (_lbwd, dict(dx=None, dw=None, db=None, ws=None, n=0), 0, ""),
     (_lbwd, dict(M=0, dw=None, db=None, dy=None), 0, ""),
-    (_gbwd, dict(zg=None), 1, "null"), (_gbwd, dict(wg=None), 1, "null"), (_gbwd, dict(ldz=31), 1, "stride"),
+    (_gbwd, dict(zg=None), 1, "null"), (_gbwd, dict(wg=None), 1, "null"), 
     (_gbwd, dict(lddw=60, dwg=None), 1, "stride"), (_gbwd, dict(ddt=-1, dbg=None), 1, "db_dtype"),
     (_gbwd, dict(ws=None), 4, "needs"), (_gbwd, dict(dt=3), 1, "dtype"),
     (_gbwd, dict(dx=None, dw=None, dwg=None, db=None, dbg=None, ws=None, n=0), 0, ""),
@@ -243,6 +243,7 @@ def test_workspace_queries_cover_padded_operands():
     if so is None:
         pytest.skip("library not built")
     M, N, K = 4096, 4096, 2048
+    assert so.dc_saved16_bytes(5, 7) == 105 and so.dc_saved16_bytes(0, 7) == 0
     q = so.dc_linear16_workspace_bytes
     assert q(P, K, P, K, M, N, K) == 0
     assert q(P + 2, K, P, K, M, N, K) == 2 * M * K
