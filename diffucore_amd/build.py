@@ -18,7 +18,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libdiffucore_amd.so"
-SOURCES = ["quant.hip", "qknorm.hip", "gemm.hip", "attn.hip", "linear16_fwd.hip", "linear16_bwd.hip", "act16.hip", "norm.hip", "calib.hip", "capi.cpp"]
+SOURCES = ["quant.hip", "qknorm.hip", "gemm.hip", "attn.hip", "linear16_fwd.hip", "linear16_bwd.hip",
+           "skinny16.hip", "act16.hip", "norm.hip", "calib.hip", "capi.cpp"]
 ARCH = "gfx950"
 
 FLAGS = [

@@ -96,6 +96,10 @@ __device__ __forceinline__ void store_saved8(uint8_t* z, int64_t M, int64_t N, i
   store_chunk16(reinterpret_cast<uint16_t*>(z) + m * N + n, N - n, make_uint4(h[0], h[1], h[2], h[3]));
   store_chunk8(z + 2 * M * N + m * N + n, N - n, make_uint2(l[0], l[1]));
 }
+__device__ __forceinline__ void store_saved1(uint8_t* z, int64_t M, int64_t N, int64_t at, float f) {
+  reinterpret_cast<uint16_t*>(z)[at] = (uint16_t)(__float_as_uint(f) >> 16);
+  z[2 * M * N + at] = (uint8_t)(__float_as_uint(f) >> 8);
+}
 __device__ __forceinline__ void load_saved8(const uint8_t* z, int64_t M, int64_t N, int64_t m, int64_t n,
                                             float (&f)[8]) {
   const uint4 u = load_chunk16(reinterpret_cast<const uint16_t*>(z) + m * N + n, N - n);

@@ -678,6 +678,19 @@ inline int pad_operand(const char* who, const Mat16& from, const Mat16& to, hipS
   return pad_rows16(who, from.p, from.ld, const_cast<void*>(to.p), from.rows, from.width, st);
 }
 
+// Whether a forward product (`rows` weight rows, of all its weights) runs on the
+// kernel for few rows of x: at most 16, and, as one launch without partial sums
+// is its gain, not where a workgroup's chain of k steps gets long or the weights'
+// bytes swamp a launch. Over 1500 random products of 1 to 16 rows the rule is
+// 1.3% off the better of the two (always this kernel 7.8%, never 8.6%): 1 x 1024
+// -> 256 8.0 us (tiles 10.5), 1 x 4096 -> 4096 8.9 (11.5); 16 x 8192 -> 1024 17.0
+// (11.9), 1 x 2048 -> 2 x 8192 15.1 (13.8).
+inline bool skinny16(int64_t M, int64_t rows, int64_t K, bool gated) {
+  return M <= 16 && rows * K <= 24 * 1000 * 1000 && (gated ? 2 : 1) * K <= (M <= 8 ? 10240 : 5120);
+}
+// It reads its operands in place at any alignment.
+int run_skinny16(const char* who, const Gemm16& p, int dtype, hipStream_t st);
+
 int refuse(int code, const char* who, const char* msg);
 // What every product checks: sizes, type, activation.
 int check_product(const char* who, int dtype, int act, int64_t M, int64_t N, int64_t K);

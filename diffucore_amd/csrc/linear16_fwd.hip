@@ -84,10 +84,12 @@ Plan16 plan16(int64_t M, int64_t rows, int64_t nk, int problems) {
 struct Forward16 {
   Mat16 x, w, w2, xs, ws, w2s;   // as given, and as the kernel reads them
   Plan16 plan;
-  float* part;
-  size_t bytes;
+  float* part = nullptr;
+  size_t bytes = 0;
+  bool skinny;
   Forward16(const Mat16& x_, const Mat16& w_, const Mat16& w2_, int64_t M, int64_t N, int64_t K, void* base)
-      : x(x_), w(w_), w2(w2_) {
+      : x(x_), w(w_), w2(w2_), xs(x_), ws(w_), w2s(w2_), skinny(skinny16(M, w2_.p ? 2 * N : N, K, w2_.p)) {
+    if (skinny) return;
     Scratch16 s{static_cast<uint8_t*>(base)};
     xs = s.operand(x), ws = s.operand(w), w2s = w2.p ? s.operand(w2) : w2;
     const int64_t rows = w2.p ? 2 * N : N;
@@ -96,6 +98,7 @@ struct Forward16 {
     bytes = s.used;
   }
   int pad(const char* who, hipStream_t st) const {
+    if (skinny) return DC_OK;
     if (int e = pad_operand(who, x, xs, st)) return e;
     if (int e = pad_operand(who, w, ws, st)) return e;
     return w2.p ? pad_operand(who, w2, w2s, st) : DC_OK;
@@ -106,7 +109,8 @@ struct Forward16 {
     p.w = static_cast<const uint16_t*>(ws.p), p.ldw = ws.ld;
     p.w2 = static_cast<const uint16_t*>(w2s.p), p.ldw2 = w2s.ld;
     // zeros past K where K is not a multiple of 8: the contraction runs over them
-    p.M = (int)M, p.N = (int)N, p.K = p.ka = (int)round_up(K, 8), p.nk = p.nk1 = (int)(round_up(K, 64) / 64);
+    p.K = p.ka = (int)(skinny ? K : round_up(K, 8));
+    p.M = (int)M, p.N = (int)N, p.nk = p.nk1 = (int)(round_up(K, 64) / 64);
     p.alim = (int)M, p.wlim = (int)N, p.problems = 1, p.part = part, p.width = (int)(w2.p ? 2 * N : N);
     return p;
   }
@@ -142,6 +146,7 @@ extern "C" int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ld
   Gemm16 p = f.args(M, N, K);
   p.bias = bias, p.bias_dtype = bias_dtype, p.act = act, p.res = static_cast<const uint16_t*>(res), p.ldr = ldr;
   p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = static_cast<uint8_t*>(z);
+  if (f.skinny) return run_skinny16(who, p, dtype, st);
   return dtype == DC_BF16 ? run_tile16<DC_BF16, false, false, EPI_LINEAR>(who, p, f.plan, st)
                           : run_tile16<DC_F16, false, false, EPI_LINEAR>(who, p, f.plan, st);
 }
@@ -172,6 +177,7 @@ extern "C" int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ld
   Gemm16 p = f.args(M, N, K);
   p.bias = bv, p.bias2 = bg, p.bias_dtype = bias_dtype, p.act = act;
   p.out = static_cast<uint16_t*>(out), p.ldo = ldo, p.z = static_cast<uint8_t*>(zv), p.z2 = static_cast<uint8_t*>(zg);
+  if (f.skinny) return run_skinny16(who, p, dtype, st);
   return dtype == DC_BF16 ? run_tile16<DC_BF16, false, false, EPI_GATED>(who, p, f.plan, st)
                           : run_tile16<DC_F16, false, false, EPI_GATED>(who, p, f.plan, st);
 }

@@ -198,11 +198,11 @@ def _norm(x=P, ldx=8, xdt=0, w=None, b=None, wdt=-1, y=P, ldy=8, stats=None, M=4
     (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"), (_linear, dict(ldo=31), 1, "stride"),
     (_linear, dict(res=P, ldr=8), 1, "stride"), 
     (_linear, dict(ldx=63), 1, "stride"), (_linear, dict(ldw=56), 1, "stride"),
-    (_linear, dict(K=60, ldx=60, ldw=60), 4, "needs"), (_linear, dict(ldx=68), 4, "needs"),
-    (_linear, dict(x=P + 8), 4, "needs"), (_linear, dict(x=P + 8, ws=P + 8, n=1 << 20), 4, "aligned"),
+    (_linear, dict(M=40, K=60, ldx=60, ldw=60), 4, "needs"), (_linear, dict(M=40, ldx=68), 4, "needs"),
+    (_linear, dict(M=40, x=P + 8), 4, "needs"), (_linear, dict(M=40, x=P + 8, ws=P + 8, n=1 << 20), 4, "aligned"),
     (_linear, dict(M=0, x=None), 0, ""), (_linear, dict(N=0), 0, ""),
     (_gated, dict(wg=None), 1, "null"), (_gated, dict(act=3), 1, "act"), (_gated, dict(zv=P), 1, "together"),
-    (_gated, dict(bg=P, bdt=-1), 1, "bias_dtype"), (_gated, dict(wg=P + 2), 4, "needs"),
+    (_gated, dict(bg=P, bdt=-1), 1, "bias_dtype"), (_gated, dict(M=40, wg=P + 2), 4, "needs"),
     (_gated, dict(M=0), 0, ""), (_gated, dict(K=0), 1, "bad M/N/K"), (_gated, dict(dt=2), 1, "dtype"),
     (_lbwd, dict(z=None), 1, "null"), (_lbwd, dict(dy=None), 1, "null"), (_lbwd, dict(ldy=31), 1, "stride"),
     (_lbwd, dict(lddx=60), 1, "stride"), (_lbwd, dict(lddw=60), 1, "stride"),
