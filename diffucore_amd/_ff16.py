@@ -170,7 +170,7 @@ def _norm_forward(x, weight, bias, eps, keep: bool):
     x2 = _flat(x)
     M, D = x2.shape
     weight, bias = _contig(weight), _contig(bias)
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2, M), device=x.device, dtype=torch.float32) if keep else None
     with _lib.device_ctx(x.device):
         rc = so.dc_layer_norm(x2.data_ptr(), x2.stride(0), _code(x2), _ptr(weight), _ptr(bias),
@@ -197,7 +197,7 @@ class _LayerNorm(torch.autograd.Function):
         x2, dy2, dev = _flat(x), _flat(dy), x.device
         M, D = x2.shape
         weight = _contig(weight)
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if want_x else None
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
         dw = torch.empty(D, device=dev, dtype=ctx.param_dtype) if want_w else None
         db = torch.empty(D, device=dev, dtype=ctx.param_dtype) if want_b else None
         with _lib.device_ctx(dev):
@@ -280,7 +280,7 @@ class _LinearAct(torch.autograd.Function):
             return None, None, None, dres, None
         so, dev, dt = _lib.require(), x.device, x.dtype
         N, K = weight.shape
-        dx = torch.empty(x.shape, device=dev, dtype=dt) if want_x else None
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
         dw = torch.empty((N, K), device=dev, dtype=dt) if want_w else None
         db = torch.empty(N, device=dev, dtype=ctx.bias_dtype) if want_b else None
         M = x.numel() // K
@@ -395,7 +395,7 @@ class _GatedLinear(torch.autograd.Function):
         fused = gate_weight is None
         rows = weight.shape[0]
         N = rows // 2 if fused else rows
-        dx = torch.empty(x.shape, device=dev, dtype=dt) if want_x else None
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want_x else None
         dw = torch.empty((rows, K), device=dev, dtype=dt) if want_w else None
         dwg = torch.empty((N, K), device=dev, dtype=dt) if want_wg else None
         db = torch.empty(rows, device=dev, dtype=ctx.bias_dtype) if want_b else None

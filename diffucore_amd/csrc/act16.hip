@@ -185,20 +185,27 @@ int act16_bwd(const char* who, const ActBwd& a, hipStream_t st) {
 
 // ---------------------------------------------------------------- padded copies
 
-// dst [M, W rounded up to 8] = src [M, W] and zeros: a thread a chunk of 8.
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* src, int64_t lds, uint16_t* dst, int64_t M,
-                                                       int W) {
-  const int64_t chunks = (W + 7) / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * chunks) return;
+// dst [rows, W rounded up to 8] = src [rows, W] and zeros, for each job: a thread
+// a chunk of 8.
+__global__ void __launch_bounds__(256) pad_rows_kernel(PadJobs p) {
+  const int j = p.count > 2 && blockIdx.x >= p.first[2] ? 2 : p.count > 1 && blockIdx.x >= p.first[1] ? 1 : 0;
+  const PadJob job = j == 0 ? p.job[0] : j == 1 ? p.job[1] : p.job[2];
+  const uint32_t first = j == 0 ? 0u : j == 1 ? p.first[1] : p.first[2];
+  const int64_t chunks = (job.width + 7) / 8, i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+  if (i >= job.rows * chunks) return;
   const int64_t r = i / chunks, c = i % chunks;
-  *reinterpret_cast<uint4*>(dst + 8 * i) = load_chunk16(src + r * lds + 8 * c, W - 8 * c);
+  reinterpret_cast<uint4*>(job.dst)[i] = load_chunk16(job.src + r * job.ld + 8 * c, job.width - 8 * c);
 }
 
-int pad_rows16(const char* who, const void* src, int64_t lds, void* dst, int64_t M, int64_t W, hipStream_t st) {
-  const int64_t n = M * ((W + 7) / 8);
-  if (n > 0x7fffffffLL * 256) return fail(DC_EINVAL, "pad_rows16: operand too large");
-  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
-                     static_cast<const uint16_t*>(src), lds, static_cast<uint16_t*>(dst), M, (int)W);
+int PadJobs::run(const char* who, hipStream_t st) {
+  if (!count) return DC_OK;
+  int64_t blocks = 0;
+  for (int j = 0; j < count; ++j) {
+    first[j] = (uint32_t)blocks;
+    blocks += (job[j].rows * ((job[j].width + 7) / 8) + 255) / 256;
+    if (blocks > 0x7fffffff) return fail(DC_EINVAL, "linear16: operands too large to pad");
+  }
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st, *this);
   return launch_status(who);
 }
 

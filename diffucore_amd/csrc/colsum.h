@@ -30,8 +30,19 @@ struct ActBwd {
 int act16_bwd(const char* who, const ActBwd& a, hipStream_t st);
 size_t act16_bwd_part_bytes(int64_t M, int64_t N, bool gated);
 
-// dst [M, W rounded up to 8] (16-byte aligned) = src [M, W] and zeros.
-int pad_rows16(const char* who, const void* src, int64_t lds, void* dst, int64_t M, int64_t W, hipStream_t st);
+// Up to three copies dst [rows, width rounded up to 8] (16-byte aligned) = src
+// [rows, width] (any alignment) and zeros, in one launch.
+struct PadJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t ld, rows, width;
+};
+struct PadJobs {
+  PadJob job[3];
+  uint32_t first[3];
+  int count = 0;
+  int run(const char* who, hipStream_t st);
+};
 
 inline bool float_dtype(int dt) { return dt == DC_F16 || dt == DC_BF16 || dt == DC_F32; }
 

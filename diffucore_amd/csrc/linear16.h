@@ -672,10 +672,11 @@ struct Scratch16 {
     return {take(2 * (size_t)m.rows * (size_t)w8), w8, m.rows, w8};
   }
 };
-// Fills an operand's padded copy, if it has one.
-inline int pad_operand(const char* who, const Mat16& from, const Mat16& to, hipStream_t st) {
-  if (to.p == from.p || from.rows == 0) return DC_OK;
-  return pad_rows16(who, from.p, from.ld, const_cast<void*>(to.p), from.rows, from.width, st);
+// Adds an operand's padded copy, if it has one, to those a call makes.
+inline void add_pad(PadJobs& jobs, const Mat16& from, const Mat16& to) {
+  if (to.p == from.p || from.rows == 0) return;
+  jobs.job[jobs.count++] = {static_cast<const uint16_t*>(from.p), static_cast<uint16_t*>(const_cast<void*>(to.p)),
+                            from.ld, from.rows, from.width};
 }
 
 // Whether a forward product (`rows` weight rows, of all its weights) runs on the

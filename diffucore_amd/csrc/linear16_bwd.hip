@@ -11,12 +11,13 @@ struct Backward16 {
   Plan16 dx_plan, dw_plan;
   float* part;
   int problems;
+  bool z;
   size_t bytes;
 
   // want_dx / want_dw / want_db as the call asks; z: there are pre-activations
-  Backward16(const Mat16& dy_, const Mat16& x_, const Mat16& wv_, const Mat16& wg_, bool z, bool want_dx, int want_dw,
+  Backward16(const Mat16& dy_, const Mat16& x_, const Mat16& wv_, const Mat16& wg_, bool z_, bool want_dx, int want_dw,
              bool want_db, void* base)
-      : dy(dy_), x(x_), wv(wv_), wg(wg_) {
+      : dy(dy_), x(x_), wv(wv_), wg(wg_), z(z_) {
     const int64_t M = dy.rows, N = dy.width, K = x.width, N64 = round_up(N, 64);
     const bool gated = wg.p;
     Scratch16 s{static_cast<uint8_t*>(base)};
@@ -42,13 +43,17 @@ struct Backward16 {
     part = static_cast<float*>(s.take(most));
     bytes = s.used;
   }
+  int pad(const char* who, hipStream_t st) const {
+    PadJobs jobs;
+    add_pad(jobs, x, xs), add_pad(jobs, wv, wvs);
+    if (wg.p) add_pad(jobs, wg, wgs);
+    else if (!z) add_pad(jobs, dy, dz);
+    return jobs.run(who, st);
+  }
   static size_t max_of(size_t a, size_t b) { return a > b ? a : b; }
 };
 
 static int run_dx(const char* who, const Backward16& b, void* dx, int64_t lddx, int dtype, hipStream_t st) {
-  if (int e = pad_operand(who, b.wv, b.wvs, st)) return e;
-  if (b.wg.p)
-    if (int e = pad_operand(who, b.wg, b.wgs, st)) return e;
   const int64_t M = b.dy.rows, N = b.dy.width, K = b.x.width, N64 = round_up(N, 64);
   Gemm16 p{};
   p.a = static_cast<const uint16_t*>(b.dz.p), p.a2 = static_cast<const uint16_t*>(b.dzg.p), p.lda = b.dz.ld;
@@ -124,17 +129,15 @@ extern "C" int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int6
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const Backward16 b({dy, lddy, M, N}, {x, ldx, M, K}, {w, ldw, N, K}, {}, act_z, dx, dw ? 1 : 0, db, ws);
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
+  if (int e = b.pad(who, st)) return e;
   if (act_z || db) {
     const ActBwd a{dy, lddy, static_cast<const uint8_t*>(act_z ? z : nullptr), nullptr, act, const_cast<void*>(act_z ? b.dz.p : nullptr),
                    nullptr, round_up(N, 64), db, nullptr, db_dtype, dtype, M, N, b.part};
     if (int e = act16_bwd(who, a, st)) return e;
   }
-  if (!act_z && (dx || dw))
-    if (int e = pad_operand(who, b.dy, b.dz, st)) return e;
   if (dx)
     if (int e = run_dx(who, b, dx, lddx, dtype, st)) return e;
   if (!dw) return DC_OK;
-  if (int e = pad_operand(who, b.x, b.xs, st)) return e;
   return run_dw(who, b, b.dz.p, dw, nullptr, nullptr, lddw, dtype, st);
 }
 
@@ -174,13 +177,13 @@ extern "C" int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64
   const Backward16 b({dy, lddy, M, N}, {x, ldx, M, K}, {wv, ldwv, N, K}, {wg, ldwg, N, K}, true, dx, dws, dbv || dbg,
                      ws);
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
+  if (int e = b.pad(who, st)) return e;
   const ActBwd a{dy, lddy, static_cast<const uint8_t*>(zv), static_cast<const uint8_t*>(zg), act, const_cast<void*>(b.dz.p), const_cast<void*>(b.dzg.p), b.dz.ld, dbv, dbg,
                  db_dtype, dtype, M, N, b.part};
   if (int e = act16_bwd(who, a, st)) return e;
   if (dx)
     if (int e = run_dx(who, b, dx, lddx, dtype, st)) return e;
   if (!dws) return DC_OK;
-  if (int e = pad_operand(who, b.x, b.xs, st)) return e;
   if (dws == 2) return run_dw(who, b, b.dz.p, dwv, b.dzg.p, dwg, lddw, dtype, st);
   return run_dw(who, b, dwv ? b.dz.p : b.dzg.p, dwv ? dwv : dwg, nullptr, nullptr, lddw, dtype, st);
 }

@@ -98,10 +98,10 @@ struct Forward16 {
     bytes = s.used;
   }
   int pad(const char* who, hipStream_t st) const {
-    if (skinny) return DC_OK;
-    if (int e = pad_operand(who, x, xs, st)) return e;
-    if (int e = pad_operand(who, w, ws, st)) return e;
-    return w2.p ? pad_operand(who, w2, w2s, st) : DC_OK;
+    PadJobs jobs;
+    add_pad(jobs, x, xs), add_pad(jobs, w, ws);
+    if (w2.p) add_pad(jobs, w2, w2s);
+    return jobs.run(who, st);
   }
   Gemm16 args(int64_t M, int64_t N, int64_t K) const {
     Gemm16 p{};
