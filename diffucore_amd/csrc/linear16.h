@@ -66,9 +66,8 @@ struct Tile16 {
   static constexpr int BN = 32 * WN * FN, BM = 32 * WM * FM;
   static constexpr int STAGE = (BN + BM) * 128;    // bytes
   static constexpr int LW = BN / 8 / NW, LA = BM / 8 / NW;   // DMA instructions per wave and stage
-  static constexpr int LDS = S * STAGE + BN * 4;
+  static constexpr int LDS = S * STAGE;
   static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole DMA instructions per wave");
-  static_assert(BN <= NT, "one bias entry per thread");
   static_assert(LDS <= 160 * 1024, "LDS per CU");
 };
 
@@ -247,13 +246,17 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
     kend = min(kt + p.kstages, p.nk);
   }
 
-  float bias = 0.0f;
+  // The bias of W row `lane` of the wave's 64 (gated: 32 value, then 32 gate
+  // rows), as loaded: issued ahead of the operands, converted after the main loop.
+  uint32_t bias_raw = 0u;
   if constexpr (EPI != EPI_NONE) {
-    if (t < BN && (p.bias || p.bias2)) {
-      // row t of the tile's W: channel, and (gated) whether of the gate
-      const int blk = t / 32;
-      const int n = GATED ? n0 + blk / 2 * 32 + t % 32 : n0 + t;
-      bias = bias_at(GATED && (blk & 1) ? p.bias2 : p.bias, p.bias_dtype, min(n, p.N - 1));
+    static_assert(FN == 2, "a lane per W row of the wave");
+    const void* b = GATED && hf ? p.bias2 : p.bias;
+    const int n = min(GATED ? n0 + 32 * wn + l32 : n0 + 64 * wn + lane, p.N - 1);
+    if (p.bias_dtype == DC_F32) {
+      if (b) bias_raw = static_cast<const uint32_t*>(b)[n];
+    } else {
+      if (b) bias_raw = static_cast<const uint16_t*>(b)[n];
     }
   }
 
@@ -452,11 +455,6 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
     }
   }
   __syncthreads();   // every wave is done reading the ring
-  float* b_l = reinterpret_cast<float*>(smem + S * T::STAGE);
-  if constexpr (EPI != EPI_NONE) {
-    if (t < BN) b_l[t] = bias;
-    __syncthreads();
-  }
 
   // epilogue
   constexpr int WAVE_BYTES = S * T::STAGE / T::NW / 16 * 16;
@@ -480,15 +478,18 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
     return;
   }
   if constexpr (EPI != EPI_NONE) {
-    // each lane's 8 columns are the same in every step: their biases once
-    float bv[8], bg[8];
+    // the wave's biases through the end of its LDS share; each lane's 8 columns
+    // are the same in every step
     constexpr int CH = GATED ? 2 * FN : 4 * FN;   // output chunks of a row
-    const int oc = lane % CH, brow = GATED ? wn * 32 * FN + oc / 4 * 64 + oc % 4 * 8 : wn * 32 * FN + oc * 8;
+    static_assert(32 * (32 * FN * 4 + 16) + 256 <= WAVE_BYTES, "the biases follow a staged block");
+    const int oc = lane % CH;
+    float* b_l = reinterpret_cast<float*>(share + WAVE_BYTES - 256);
+    asm volatile("" : "+v"(bias_raw));   // not converted, and waited for, where it is loaded
+    b_l[lane] = p.bias_dtype == DC_F32 ? __uint_as_float(bias_raw) : h16_to_f32<DT>(bias_raw);
+    wave_lds_fence();
+    float bv[8], bg[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bv[e] = b_l[brow + e];
-      if constexpr (GATED) bg[e] = b_l[brow + 32 + e];
-    }
+    for (int e = 0; e < 8; ++e) bv[e] = b_l[8 * oc + e], bg[e] = GATED ? b_l[32 + 8 * oc + e] : 0.0f;
     const int n = nb + 8 * oc;
     // one uniform branch around the whole of it, so that the steps of a block overlap
     with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
@@ -614,12 +615,15 @@ typedef Tile16<4, 2, 2, 4, 2, 2> T256x256;    // 8 waves of 64 x 128, 128 KB: 1 
 typedef Tile16<4, 2, 2, 3, 2, 2> T256x192;    // 8 waves of 64 x 96, 112 KB: 1 per CU
 typedef Tile16<4, 2, 2, 2, 3, 2> T256x128;    // 8 waves of 64 x 64, 144 KB: 1 per CU
 typedef Tile16<2, 4, 2, 2, 3, 2> T128x256;    // 8 waves of 64 x 64, 144 KB: 1 per CU
+typedef Tile16<2, 2, 2, 3, 2, 2> T128x192;    // 4 waves of 64 x 96, 80 KB: 2 per CU
 typedef Tile16<2, 2, 2, 2, 2, 2> T128x128;    // 4 waves of 64 x 64, 64 KB: 2 per CU
 typedef Tile16<2, 4, 2, 1, 3, 2> T128x128d;   // 8 waves of 64 x 32, 96 KB: 1 per CU
 typedef Tile16<1, 4, 2, 1, 3, 2> T64x128;     // 4 waves of 64 x 32, 72 KB: 2 per CU
 typedef Tile16<1, 2, 2, 1, 3, 2> T64x64;      // 2 waves of 64 x 32, 48 KB: 3 per CU
-enum { TILE_256x256 = 0, TILE_128x128 = 1, TILE_128x128D = 2, TILE_64x128 = 3, TILE_64x64 = 4, TILE_256x192 = 5,
-       TILE_256x128 = 6, TILE_128x256 = 7 };
+enum {
+  TILE_256x256, TILE_256x192, TILE_256x128, TILE_128x256, TILE_128x192, TILE_128x128, TILE_128x128D, TILE_64x128,
+  TILE_64x64
+};
 
 template <int DT, bool A_RC, bool W_RC, int EPI>
 int run_tile16(const char* who, const Gemm16& p, const Plan16& plan, hipStream_t st) {
@@ -628,6 +632,7 @@ int run_tile16(const char* who, const Gemm16& p, const Plan16& plan, hipStream_t
     case TILE_256x192: return launch16<T256x192, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_256x128: return launch16<T256x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_128x256: return launch16<T128x256, DT, A_RC, W_RC, EPI>(who, p, plan, st);
+    case TILE_128x192: return launch16<T128x192, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_128x128: return launch16<T128x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_128x128D: return launch16<T128x128d, DT, A_RC, W_RC, EPI>(who, p, plan, st);
     case TILE_64x128: return launch16<T64x128, DT, A_RC, W_RC, EPI>(who, p, plan, st);

@@ -30,31 +30,33 @@ int check_scratch(const char* who, size_t need, const void* ws, size_t ws_bytes)
 }
 
 // Tile and k slices by the least of a fitted time, in us:
-//   T = fixed + h (round + stage * stages)  [+ 2.9 + 0.32 per MB of partial sums when k is split]
+//   T = fixed + h (round + stage * stages)  [+ 3.2 + 0.34 per MB of partial sums when k is split]
 // where a round fills every CU with `per` workgroups of the tile and h counts
 // rounds; a last round in which the busiest CU holds j < per of them counts
 // level[j - 1], and any level that is not full on every CU counts up to `slack`
-// less (the clock rises and memory frees as CUs fall idle). Fitted to 20000 random
+// less (the clock rises and memory frees as CUs fall idle). Fitted to 10500 random
 // products of 17 to 16384 rows, 16 to 20480 channels and 64 to 8192 of k (all
-// three operand layouts, 8 tiles, up to 16 slices; operands rotated through
-// memory): rms error of a time 9 to 13%, and the pick is 2.5% off the best of all
-// tiles and slices on average, 1.6% for products past 40 GFLOP. A rule that went
-// by the number of 128 x 128 tiles was 6.9% off. At 256 x 256 / 256 x 192 / 128 x
-// 128: 4608 x 2048 -> 8192 191 / 153 / 160 us, 8192 x 2560 -> 640 59 / 49 / 36,
-// dw of 4608 x (2048, 8192) 129 / 188 / 157.
+// three operand layouts, with and without kept pre-activations, 9 tiles, up to 16
+// slices; operands rotated through memory): rms error of a time 9 to 14%, and the
+// pick is 1.9% off the best of all tiles and slices on average. A rule that went by
+// the number of 128 x 128 tiles was 6.9% off. At 256 x 256 / 256 x 192 / 128 x 192 /
+// 128 x 128, us: 4608 x 2048 -> 8192 196 / 159 / 161 / 171, gated 8192 x 640 -> 2560
+// 76 / 80 / 68 / 72, 8192 x 2560 -> 640 62 / 51 / 41 / 38, dw of 4608 x (2048, 8192)
+// 131 / 190 / 158 / 153.
 struct TileCost {
   int tile, bn, bm, per;
   float fixed, round, stage, slack, level[2];
 };
 static constexpr TileCost COSTS[] = {
-    {TILE_256x256, 256, 256, 1, 3.25f, 7.61f, 1.791f, 0.35f, {}},
-    {TILE_256x192, 256, 192, 1, 2.98f, 5.65f, 1.527f, 0.38f, {}},
-    {TILE_256x128, 256, 128, 1, 3.39f, 4.55f, 0.997f, 0.33f, {}},
-    {TILE_128x256, 128, 256, 1, 3.32f, 4.59f, 1.007f, 0.34f, {}},
-    {TILE_128x128, 128, 128, 2, 4.08f, 3.27f, 1.053f, 0.27f, {0.78f}},
-    {TILE_128x128D, 128, 128, 1, 4.49f, 2.77f, 0.570f, 0.32f, {}},
-    {TILE_64x128, 64, 128, 2, 5.89f, 1.64f, 0.710f, 0.22f, {0.53f}},
-    {TILE_64x64, 64, 64, 3, 6.25f, 1.36f, 0.691f, 0.12f, {0.40f, 0.60f}},
+    {TILE_256x256, 256, 256, 1, 1.47f, 7.95f, 1.840f, 0.315f, {}},
+    {TILE_256x192, 256, 192, 1, 2.85f, 5.39f, 1.485f, 0.341f, {}},
+    {TILE_256x128, 256, 128, 1, 3.00f, 4.57f, 1.001f, 0.312f, {}},
+    {TILE_128x256, 128, 256, 1, 3.01f, 4.60f, 1.016f, 0.334f, {}},
+    {TILE_128x192, 128, 192, 2, 4.76f, 4.50f, 1.490f, 0.232f, {0.675f}},
+    {TILE_128x128, 128, 128, 2, 3.35f, 3.45f, 1.129f, 0.202f, {0.792f}},
+    {TILE_128x128D, 128, 128, 1, 3.83f, 2.93f, 0.586f, 0.316f, {}},
+    {TILE_64x128, 64, 128, 2, 5.21f, 1.77f, 0.768f, 0.232f, {0.549f}},
+    {TILE_64x64, 64, 64, 3, 5.75f, 1.42f, 0.671f, 0.108f, {0.395f, 0.646f}},
 };
 
 Plan16 plan16(int64_t M, int64_t rows, int64_t nk, int problems) {
@@ -73,7 +75,7 @@ Plan16 plan16(int64_t M, int64_t rows, int64_t nk, int problems) {
       float h = (float)(units / slots);
       if (j) h += (j < c.per ? c.level[j - 1] : 1.0f) * (1.0f - c.slack * (1.0f - (float)rest / (float)(cus * j)));
       float t = c.fixed + h * (c.round + c.stage * (float)stages);
-      if (splits > 1) t += 2.9f + 0.32f * mb * (float)splits;
+      if (splits > 1) t += 3.2f + 0.34f * mb * (float)splits;
       if (t < least) least = t, best = {c.tile, (int)splits, (int)stages};
     }
   }
@@ -136,7 +138,8 @@ extern "C" int dc_linear16(const void* x, int64_t ldx, const void* w, int64_t ld
   if (int e = check_product(who, dtype, act, M, N, K)) return e;
   if (M == 0 || N == 0) return DC_OK;
   if (!x || !w || !out) return refuse(DC_EINVAL, who, "null pointer");
-  if (bias && !float_dtype(bias_dtype)) return refuse(DC_EINVAL, who, "bad bias_dtype");
+  if (bias && bias_dtype != dtype && bias_dtype != DC_F32)
+    return refuse(DC_EINVAL, who, "bias_dtype must be dtype or DC_F32");
   if (ldx < K || ldw < K || ldo < N || (res && ldr < N))
     return refuse(DC_EINVAL, who, "row stride less than the row");
   const Forward16 f({x, ldx, M, K}, {w, ldw, N, K}, {}, M, N, K, ws);
@@ -166,7 +169,8 @@ extern "C" int dc_gated16(const void* x, int64_t ldx, const void* wv, int64_t ld
   if (int e = check_product(who, dtype, act, M, N, K)) return e;
   if (M == 0 || N == 0) return DC_OK;
   if (!x || !wv || !wg || !out) return refuse(DC_EINVAL, who, "null pointer");
-  if ((bv || bg) && !float_dtype(bias_dtype)) return refuse(DC_EINVAL, who, "bad bias_dtype");
+  if ((bv || bg) && bias_dtype != dtype && bias_dtype != DC_F32)
+    return refuse(DC_EINVAL, who, "bias_dtype must be dtype or DC_F32");
   if (!zv != !zg) return refuse(DC_EINVAL, who, "zv and zg go together");
   if (ldx < K || ldwv < K || ldwg < K || ldo < N)
     return refuse(DC_EINVAL, who, "row stride less than the row");

@@ -397,8 +397,8 @@ int dc_int8_attn_quantize_q(const void* q, int dtype, int B, int H, int Lq, int 
  */
 
 /*
- * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once. bias [N] of
- * bias_dtype (DC_NONE: none), res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
+ * out[M, N] = act(x[M, K] w[N, K]^T + bias) + res, rounded once. bias [N] (or
+ * NULL) of bias_dtype, which is `dtype` or DC_F32, res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
  * GELU_TANH / SILU / QUICK_GELU. z (or NULL; 2-byte aligned,
  * dc_saved16_bytes) takes the pre-activation x w^T + bias for dc_linear16_bwd:
  * the upper 24 bits of its float32 values, a plane of halves and one of bytes.
