@@ -420,15 +420,21 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
   sync();
   int slot = 0;
   if (kt + 1 < kend) frags(0, 0, 0);
+  // The first of two terms may end inside a stage too: the zeros that A holds
+  // there do not do, as 0 times an infinite w is NaN.
+  constexpr bool TERMS = W_RC && !A_RC;
+  const int mask_at = TERMS && p.nk > p.nk1 && p.K % 64 ? p.nk1 - 1 : -1;
   // stage kt in `slot`; MORE: stage kt + S exists
   auto stage = [&](auto more) __attribute__((always_inline)) {
     constexpr bool MORE = decltype(more)::value;
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks) {
+      if (TERMS && kt == mask_at) mask(ks & 1, ks, p.K % 64);
       frags((ks + 1) & 1, slot, ks + 1);
       mfmas(ks & 1);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (TERMS && kt == mask_at) mask(1, 3, p.K % 64);
     const int next = slot == S - 1 ? 0 : slot + 1;
     if constexpr (MORE) wait_vmcnt<(S - 2) * L>();
     else wait_left(kend - 2 - kt);

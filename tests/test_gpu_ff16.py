@@ -271,6 +271,29 @@ def test_infinities_and_nan_stay_in_their_rows(gpu, M):
     assert torch.equal(y[1].float(), torch.where(w[:, 3] > 0, float("inf"), float("-inf")).float())
 
 
+@pytest.mark.parametrize("F_, K", [(40, 72), (70, 200), (127, 65), (300, 264)])
+@pytest.mark.parametrize("half", [0, 1])
+def test_infinite_weights_reach_their_column_only(gpu, half, F_, K):
+    """An infinite weight in a half's last row, where the product's sum over
+    that half ends inside a stage of 64: dx's column is infinite with the sign
+    of its dz, never NaN, and the others stay as they are without it."""
+    g = _gen(12)
+    dt = torch.bfloat16
+    x = _rand(g, 70, K, dtype=dt).requires_grad_(True)
+    w = _rand(g, 2 * F_, K, dtype=dt, std=0.1)
+    dy = _rand(g, 70, F_, dtype=dt)
+    clean, = torch.autograd.grad(D.gated_linear(x, w, act="silu"), [x], dy)
+    y = D.gated_linear(x, w, act="silu")
+    v, gate = (t[:, -1] for t in (x.detach().double() @ w.double().T).chunk(2, dim=1))
+    a, slope = O.act(gate, "silu")
+    dz = dy[:, -1].double() * (v * slope if half else a)
+    w.data[(1 + half) * F_ - 1, 1] = float("inf")   # after the forward: its pre-activations stay finite
+    got, = torch.autograd.grad(y, [x], dy)
+    keep = [c for c in range(K) if c != 1]
+    assert torch.equal(got[:, keep], clean[:, keep])
+    assert torch.equal(got[:, 1].double(), torch.sign(dz) * float("inf"))
+
+
 @pytest.mark.parametrize("act", [a for a in ACTS if a != "none"])
 def test_far_out_pre_activations(gpu, act):
     """Values where x s (1 - s) or x phi(x) would turn into inf * 0: slopes
@@ -313,6 +336,75 @@ def test_gpu_refusals(gpu):
         D.linear_act(x.half(), w.half().cpu())
     with pytest.raises(ValueError, match="bias is on"):
         D.layer_norm(x, bias=torch.zeros(8))
+
+
+# ---------------------------------------------------------------- past 32 bits
+
+def test_layer_norm_past_32_bits(gpu):
+    """2.2e9 elements: the last rows equal a call on them alone."""
+    M, D_ = 270000, 8192
+    x = torch.empty(M, D_, device="cuda", dtype=torch.bfloat16)
+    x[:64].normal_()
+    x[-64:].normal_()
+    x[64:-64] = x[0]
+    w = torch.randn(D_, device="cuda")
+    y = D.layer_norm(x, w)
+    for rows in (slice(0, 64), slice(M - 64, M)):
+        assert torch.equal(y[rows], D.layer_norm(x[rows], w))
+    t = x.requires_grad_(True)
+    dx, = torch.autograd.grad(D.layer_norm(t, w), [t], y)
+    tail = x[-64:].detach().requires_grad_(True)
+    want, = torch.autograd.grad(D.layer_norm(tail, w), [tail], y[-64:])
+    assert torch.equal(dx[-64:], want)
+
+
+def test_products_past_32_bits(gpu):
+    """An input of 2.4e9 elements and, the other way round, an output of as
+    many: their last rows equal calls on those rows alone (each output is summed
+    in the same order on every tile, so the bits agree)."""
+    M, K, N = 300000, 8192, 64
+    g = _gen(13)
+    x = torch.empty(M, K, device="cuda", dtype=torch.bfloat16)
+    x[-512:] = _rand(g, 512, K, dtype=torch.bfloat16)
+    x[:-512] = x[-1]
+    w = _rand(g, N, K, dtype=torch.bfloat16, std=0.02)
+    y = D.linear_act(x, w, act="gelu")
+    f = lambda t: t.double()   # noqa: E731
+    want = O.linear(f(x[-512:]), f(w), None, "gelu", None, torch.bfloat16)
+    _within(y[-512:], want["y"], "y")
+    t = x.requires_grad_(True)
+    dy = torch.zeros(M, N, device="cuda", dtype=torch.bfloat16)
+    dy[-512:] = _rand(g, 512, N, dtype=torch.bfloat16)
+    lw = w.detach().requires_grad_(True)
+    dx, dw = torch.autograd.grad(D.linear_act(t, lw, act="gelu"), [t, lw], dy)
+    want = O.linear(f(x[-512:].detach()), f(w), None, "gelu", None, torch.bfloat16, f(dy[-512:]))
+    _within(dx[-512:], want["dx"], "dx")
+    assert not bool(dx[:-512].any())
+    _within(dw, want["dw"], "dw")   # the other rows' gradients are 0
+    del dx, t, x
+    wide = _rand(g, K, N, dtype=torch.bfloat16, std=0.1)
+    h = y.detach()
+    out = D.gated_linear(h, wide, gate_weight=wide)
+    want = O.gated(f(h[-512:]), f(wide), f(wide), None, None, "gelu", torch.bfloat16)
+    _within(out[-512:], want["y"], "gated y")
+
+
+def test_huge_row_strides(gpu):
+    """Rows 2^22 elements and more apart (32-bit offsets within a tile would not
+    reach them) are copied first."""
+    g = _gen(14)
+    big = torch.empty(40, (1 << 22) + 8, device="cuda", dtype=torch.float16)
+    big[:, :64] = _rand(g, 40, 64, dtype=torch.float16)
+    x = big[:, :64]
+    w = _rand(g, 72, 64, dtype=torch.float16, std=0.1)
+    assert torch.equal(D.linear_act(x, w, act="silu"), D.linear_act(x.contiguous(), w, act="silu"))
+    a, b = (t.detach().requires_grad_(True) for t in (x, x.contiguous()))
+    dy = _rand(g, 40, 72, dtype=torch.float16)
+    lw = w.requires_grad_(True)
+    for p, q in zip(torch.autograd.grad(D.linear_act(a, lw), [a, lw], dy),
+                    torch.autograd.grad(D.linear_act(b, lw), [b, lw], dy)):
+        assert torch.equal(p, q)
+    assert torch.equal(D.layer_norm(x), D.layer_norm(x.contiguous()))
 
 
 # ---------------------------------------------------------------- how calls are used
