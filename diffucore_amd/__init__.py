@@ -17,9 +17,11 @@ from .runtime import DevicePolicy
 __all__ = sorted([
     "GROUP", "DevicePolicy", "Int8Embedding", "Int8Linear", "act_quantize", "adopt_int8_embedding",
     "adopt_int8_layers", "attention_bhld", "attention_blhd", "dequantize_linears", "dequantize_weight",
-    "fa2_turing_available", "flux_qk_norm_rope", "fuse_linears", "gated_linear", "geglu_ff", "geglu_quantize", "gelu_quantize",
+    "fa2_turing_available", "flux_qk_norm_rope", "fuse_linears", "gated_linear", "geglu_ff",
+    "geglu_quantize", "gelu_quantize",
     "int8_attention", "int8_geglu_ff",
-    "int8_fast_available", "int8_layers", "int8_mlp", "int8_turing_available", "int_mm", "layer_norm", "linear_act", "linear_group",
+    "int8_fast_available", "int8_layers", "int8_mlp", "int8_turing_available", "int_mm", "layer_norm",
+    "linear_act", "linear_group",
     "ln_mod_quantize", "matmul_quantized_gated", "matmul_quantized_group",
     "lora_seed", "norm_rope", "qk_norm_rope", "qk_ok", "quantize_activation", "quantize_linears",
     "quantize_weight", "rescale", "resolve_attention_backend", "scaled_mm", "set_attention_backend",

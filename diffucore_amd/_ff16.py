@@ -11,6 +11,9 @@ runs torch's own ops there (``unet.py:148-183``).
 
 All of them take tensors of any leading shape and any strides, enqueue on
 torch's current stream of the tensors' device, and are differentiable once.
+They can be captured into a HIP graph after one call of the same shapes; a
+backward pass is captured as torch's own are: no eager autograd graph of the
+same leaves may be alive then (detach the leaves, or drop its outputs first).
 Sums, statistics and gradients are accumulated in float32 and rounded once; for
 the backward pass of an activation its input is kept in 24 bits, and the
 gradient at it is rounded to 16 bits as the operand of the products that follow.
@@ -62,6 +65,8 @@ def _check_input(what: str, x: torch.Tensor) -> None:
 
 
 def _check_like(what: str, name: str, t: torch.Tensor, x: torch.Tensor, shape: tuple, dtypes: tuple) -> None:
+    if t.shape == shape and t.dtype in dtypes and t.device == x.device:
+        return
     if t.device != x.device:
         raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
     if tuple(t.shape) != shape:
@@ -75,9 +80,10 @@ def _check_product(what: str, x: torch.Tensor, weight: torch.Tensor) -> None:
     if weight.dim() != 2:
         raise ValueError(f"{what}: weight is {weight.dim()}-dimensional, expected [out, in]")
     _check_like(what, "weight", weight, x, (weight.shape[0], x.shape[-1]), (x.dtype,))
-    if x.is_cuda and x.dtype not in _HALF:
-        raise TypeError(f"{what}: the kernels take fp16 or bf16 tensors, got {x.dtype}")
-    if not (x.is_cuda or _host(x)):
+    if x.is_cuda:
+        if x.dtype not in _HALF:
+            raise TypeError(f"{what}: the kernels take fp16 or bf16 tensors, got {x.dtype}")
+    elif not _host(x):
         raise RuntimeError(f"{what}: diffucore_amd runs on GPU and CPU tensors (got a {x.device} tensor)")
 
 
@@ -86,7 +92,11 @@ def _host(t: torch.Tensor) -> bool:
 
 
 def _needs_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ─── operands ────────────────────────────────────────────────────────────────
@@ -99,7 +109,7 @@ def _flat(t: torch.Tensor) -> torch.Tensor:
         t = t.reshape(-1, t.shape[-1])
     rows, width = t.shape
     step, unit = t.stride()
-    if unit == 1 and step >= width:
+    if unit == 1 and (step == width or (step > width and rows != 1)):
         return t
     if (unit != 1 and width != 1) or (rows != 1 and step < width):
         t = t.contiguous()
@@ -110,8 +120,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_CODES = {None: _lib.NONE, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
 def _code(t) -> int:
-    return _lib.NONE if t is None else _lib.dtype_code(t.dtype)
+    return _CODES[None if t is None else t.dtype]
 
 
 def _contig(t):
@@ -155,7 +168,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
             _check_like(what, name, t, x, (D,), _FLOAT)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"{what}: weight is {weight.dtype}, bias {bias.dtype}")
-    if _host(x):
+    if not x.is_cuda and _host(x):
         y = F.layer_norm(x.float(), (D,), None if weight is None else weight.float(), None, eps)
         return (y if bias is None else y + bias.float()).to(x.dtype)
     if not x.is_cuda:
@@ -176,7 +189,8 @@ def _norm_forward(x, weight, bias, eps, keep: bool):
         rc = so.dc_layer_norm(x2.data_ptr(), x2.stride(0), _code(x2), _ptr(weight), _ptr(bias),
                               _code(weight if weight is not None else bias), eps, y.data_ptr(), D, _ptr(stats), M, D,
                               _lib.stream_ptr(x.device))
-    _lib.check(rc, "dc_layer_norm")
+    if rc:
+        _lib.check(rc, "dc_layer_norm")
     return y, stats
 
 
@@ -205,11 +219,11 @@ class _LayerNorm(torch.autograd.Function):
             if want_w or want_b:
                 need = _scratch_bytes("dc_layer_norm_bwd_workspace_bytes", dev.index, M, D, _code(x))
             ws = _scratch(need, dev)
-            code = _lib.NONE if ctx.param_dtype is None else _lib.dtype_code(ctx.param_dtype)
             rc = so.dc_layer_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), _code(x),
-                                      _ptr(weight), code, stats.data_ptr(), _ptr(dx), D, _ptr(dw), _ptr(db), M, D,
-                                      _ptr(ws), need, _lib.stream_ptr(dev))
-        _lib.check(rc, "dc_layer_norm_bwd")
+                                      _ptr(weight), _CODES[ctx.param_dtype], stats.data_ptr(), _ptr(dx), D, _ptr(dw),
+                                      _ptr(db), M, D, _ptr(ws), need, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, "dc_layer_norm_bwd")
         return dx, dw, db, None
 
 
@@ -231,7 +245,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         _check_like(what, "bias", bias, x, (N,), (x.dtype, torch.float32))
     if residual is not None:
         _check_like(what, "residual", residual, x, (*x.shape[:-1], N), (x.dtype,))
-    if _host(x):
+    if not x.is_cuda:
         y = _act(F.linear(x.float(), weight.float(), None if bias is None else bias.float()), act)
         return (y if residual is None else y + residual.float()).to(x.dtype)
     if _needs_grad(x, weight, bias, residual):
@@ -241,7 +255,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
     so = _lib.require()
-    dev, dt = x.device, _lib.dtype_code(x.dtype)
+    dev, dt = x.device, _CODES[x.dtype]
     x2, w2 = _flat(x), _flat(weight)
     (M, K), N = x2.shape, w2.shape[0]
     out = torch.empty((*x.shape[:-1], N), device=dev, dtype=x.dtype)
@@ -257,7 +271,8 @@ def _linear_forward(x, weight, bias, residual, act: int, keep: bool):
         rc = so.dc_linear16(x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(bias), _code(bias), _ptr(r2),
                             0 if r2 is None else r2.stride(0), act, out.data_ptr(), N, _ptr(z), dt, M, N, K,
                             _ptr(ws), need, _lib.stream_ptr(dev))
-    _lib.check(rc, "dc_linear16")
+    if rc:
+        _lib.check(rc, "dc_linear16")
     return out, z
 
 
@@ -294,9 +309,10 @@ class _LinearAct(torch.autograd.Function):
                                   ldw, ctx.act, want, M, N, K)
             ws = _scratch(need, dev)
             rc = so.dc_linear16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(z), ctx.act,
-                                    _ptr(dx), K, _ptr(dw), K, _ptr(db), _code(db), _lib.dtype_code(dt), M, N, K,
+                                    _ptr(dx), K, _ptr(dw), K, _ptr(db), _code(db), _CODES[dt], M, N, K,
                                     _ptr(ws), need, _lib.stream_ptr(dev))
-        _lib.check(rc, "dc_linear16_bwd")
+        if rc:
+            _lib.check(rc, "dc_linear16_bwd")
         return dx, dw, db, dres, None
 
 
@@ -327,7 +343,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
             _check_like(what, name, t, x, (N,), bias_types)
     if bias is not None and gate_bias is not None and bias.dtype != gate_bias.dtype:
         raise TypeError(f"{what}: bias is {bias.dtype}, gate_bias {gate_bias.dtype}")
-    if _host(x):
+    if not x.is_cuda:
         xf = x.float()
         if gate_weight is None:
             v, g = F.linear(xf, weight.float(), None if bias is None else bias.float()).chunk(2, dim=-1)
@@ -372,9 +388,10 @@ def _gated_forward(x, weight, bias, gate_weight, gate_bias, act: int, keep: bool
         ws = _scratch(need, dev)
         rc = so.dc_gated16(x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, bv, bg,
                            _code(bias if bias is not None else gate_bias), act, out.data_ptr(), N, zv,
-                           None if z is None else zv + half, _lib.dtype_code(x.dtype), M, N, K, _ptr(ws), need,
+                           None if z is None else zv + half, _CODES[x.dtype], M, N, K, _ptr(ws), need,
                            _lib.stream_ptr(dev))
-    _lib.check(rc, "dc_gated16")
+    if rc:
+        _lib.check(rc, "dc_gated16")
     return out, z
 
 
@@ -383,7 +400,8 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, gate_weight, gate_bias, act):
         y, z = _gated_forward(x, weight, bias, gate_weight, gate_bias, act, True)
         ctx.save_for_backward(x, weight, gate_weight, z)
-        ctx.act, ctx.bias_dtype = act, bias.dtype if bias is not None else None if gate_bias is None else gate_bias.dtype
+        either = bias if bias is not None else gate_bias
+        ctx.act, ctx.bias_dtype = act, None if either is None else either.dtype
         return y
 
     @staticmethod
@@ -415,14 +433,15 @@ class _GatedLinear(torch.autograd.Function):
                 + (want_b or want_bg) * _WANT_DB)
         zv = z.data_ptr()
         with _lib.device_ctx(dev):
-            need = _scratch_bytes("dc_gated16_bwd_workspace_bytes", dev.index, _at(dy2), ldy, _at(x2), ldx, _at(wv), ldv,
-                                  _at(wg), ldg, want, M, N, K)
+            need = _scratch_bytes("dc_gated16_bwd_workspace_bytes", dev.index, _at(dy2), ldy, _at(x2), ldx, _at(wv),
+                                  ldv, _at(wg), ldg, want, M, N, K)
             ws = _scratch(need, dev)
             rc = so.dc_gated16_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, wv.data_ptr(), ldv, wg.data_ptr(), ldg, zv,
                                    zv + z.numel() // 2, ctx.act, _ptr(dx), K, dwv_p, dwg_p, K, dbv_p, dbg_p,
-                                   _lib.NONE if ctx.bias_dtype is None else _lib.dtype_code(ctx.bias_dtype),
-                                   _lib.dtype_code(dt), M, N, K, _ptr(ws), need, _lib.stream_ptr(dev))
-        _lib.check(rc, "dc_gated16_bwd")
+                                   _CODES[ctx.bias_dtype],
+                                   _CODES[dt], M, N, K, _ptr(ws), need, _lib.stream_ptr(dev))
+        if rc:
+            _lib.check(rc, "dc_gated16_bwd")
         return dx, dw, db, dwg, dbg, None
 
 

@@ -209,7 +209,8 @@ __device__ __forceinline__ float4 load_chunk32(const float* p, int64_t n) {
 }
 __device__ __forceinline__ void store_chunk32(float* p, int64_t n, float4 f) {
   if (n >= 4) {
-    store_words<float, 4>(p, {{__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)}});
+    store_words<float, 4>(p, {{__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z),
+                               __float_as_uint(f.w)}});
     return;
   }
   if (n > 0) p[0] = f.x;

@@ -131,8 +131,9 @@ extern "C" int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int6
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
   if (int e = b.pad(who, st)) return e;
   if (act_z || db) {
-    const ActBwd a{dy, lddy, static_cast<const uint8_t*>(act_z ? z : nullptr), nullptr, act, const_cast<void*>(act_z ? b.dz.p : nullptr),
-                   nullptr, round_up(N, 64), db, nullptr, db_dtype, dtype, M, N, b.part};
+    const ActBwd a{dy, lddy, static_cast<const uint8_t*>(act_z ? z : nullptr), nullptr, act,
+                   const_cast<void*>(act_z ? b.dz.p : nullptr), nullptr, round_up(N, 64), db, nullptr, db_dtype, dtype,
+                   M, N, b.part};
     if (int e = act16_bwd(who, a, st)) return e;
   }
   if (dx)
@@ -178,8 +179,9 @@ extern "C" int dc_gated16_bwd(const void* dy, int64_t lddy, const void* x, int64
                      ws);
   if (int e = check_scratch(who, b.bytes, ws, ws_bytes)) return e;
   if (int e = b.pad(who, st)) return e;
-  const ActBwd a{dy, lddy, static_cast<const uint8_t*>(zv), static_cast<const uint8_t*>(zg), act, const_cast<void*>(b.dz.p), const_cast<void*>(b.dzg.p), b.dz.ld, dbv, dbg,
-                 db_dtype, dtype, M, N, b.part};
+  const ActBwd a{dy, lddy, static_cast<const uint8_t*>(zv), static_cast<const uint8_t*>(zg), act,
+                 const_cast<void*>(b.dz.p), const_cast<void*>(b.dzg.p), b.dz.ld, dbv, dbg, db_dtype, dtype, M, N,
+                 b.part};
   if (int e = act16_bwd(who, a, st)) return e;
   if (dx)
     if (int e = run_dx(who, b, dx, lddx, dtype, st)) return e;

@@ -585,6 +585,6 @@ extern "C" int dc_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, in
   p.part = sums ? static_cast<float*>(ws) : nullptr;
   p.ldx = ldx, p.lddy = lddy, p.ldo = lddx, p.M = M, p.D = (int)D, p.w_dtype = w_dtype;
   if (int e = dispatch_norm(p, x_dtype, true, st)) return e;
-  return sums ? reduce_partials(p.part, (int)bwd_blocks(M, norm_plan(D, x_dtype), x_dtype), 2, D, dw, db, w_dtype, st, who)
-              : DC_OK;
+  const int64_t P = bwd_blocks(M, norm_plan(D, x_dtype), x_dtype);
+  return sums ? reduce_partials(p.part, (int)P, 2, D, dw, db, w_dtype, st, who) : DC_OK;
 }

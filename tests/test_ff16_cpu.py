@@ -195,7 +195,8 @@ def _norm(x=P, ldx=8, xdt=0, w=None, b=None, wdt=-1, y=P, ldy=8, stats=None, M=4
     (_linear, dict(N=1 << 29), 1, "too large"), (_linear, dict(K=1 << 22, ldx=1 << 22), 1, "too large"),
     (_linear, dict(dt=2), 1, "dtype"), (_linear, dict(act=3), 1, "act"), (_linear, dict(K=0), 1, "bad M/N/K"),
     (_linear, dict(x=None), 1, "null"), (_linear, dict(out=None), 1, "null"),
-    (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"), (_linear, dict(bias=P, bdt=0, dt=1), 1, "bias_dtype"), (_linear, dict(ldo=31), 1, "stride"),
+    (_linear, dict(bias=P, bdt=3), 1, "bias_dtype"), (_linear, dict(bias=P, bdt=0, dt=1), 1, "bias_dtype"),
+    (_linear, dict(ldo=31), 1, "stride"),
     (_linear, dict(res=P, ldr=8), 1, "stride"), 
     (_linear, dict(ldx=63), 1, "stride"), (_linear, dict(ldw=56), 1, "stride"),
     (_linear, dict(M=40, K=60, ldx=60, ldw=60), 4, "needs"), (_linear, dict(M=40, ldx=68), 4, "needs"),

@@ -148,8 +148,8 @@ def test_gated_rows(gpu, M, fused, dt):
     _check_gated(M, 320, 272, dt, "gelu", fused=fused, seed=M)
 
 
-@pytest.mark.parametrize("K, N", [(8, 8), (1, 1), (5, 3), (16, 2), (40, 72), (63, 65), (64, 32), (127, 257), (1000, 2731),
-                                  (2560, 640), (24, 2000)])
+@pytest.mark.parametrize("K, N", [(8, 8), (1, 1), (5, 3), (16, 2), (40, 72), (63, 65), (64, 32), (127, 257),
+                                  (1000, 2731), (2560, 640), (24, 2000)])
 @pytest.mark.parametrize("M", [1, 19, 260])
 def test_gated_widths(gpu, M, K, N):
     act = [a for a in ACTS if a != "none"][(K + N) % 4]
@@ -318,7 +318,8 @@ def test_empty_calls(gpu):
     b = torch.randn(6, device="cuda", dtype=torch.float16).requires_grad_(True)
     x = torch.zeros(0, 8, device="cuda", dtype=torch.float16).requires_grad_(True)
     r = torch.zeros(0, 6, device="cuda", dtype=torch.float16).requires_grad_(True)
-    for y, leaves in ((D.linear_act(x, w, b, act="silu", residual=r), [x, w, b, r]), (D.gated_linear(x, w, b), [x, w, b]),
+    for y, leaves in ((D.linear_act(x, w, b, act="silu", residual=r), [x, w, b, r]),
+                      (D.gated_linear(x, w, b), [x, w, b]),
                       (D.layer_norm(x, w[0], b[:1].expand(8)), [x, w, b])):
         assert y.shape[0] == 0
         for t, grad in zip(leaves, torch.autograd.grad(y, leaves, torch.zeros_like(y))):
@@ -534,3 +535,31 @@ def test_sublayer(gpu, M):
     for i, (a, b) in enumerate([(y, yd), *zip(got, want)]):
         rel = float((a.detach().double() - b.detach()).norm() / b.detach().norm())
         assert rel < 6 * 2.0 ** -8, (i, rel)
+
+
+@pytest.mark.parametrize("level", [0, 2])
+def test_unet_block_trains_as_eager(gpu, level):
+    """The UNet block on these operators (``unet_block.to_fused16``) against the
+    eager fp16 block: output and every gradient. Both round at every op, the
+    eager one at more of them (norm, projection, gelu, product, sum: 5 to our
+    3), so the two differ by at most the sum of both, taken as 16 half steps in
+    relative L2 (a chain of three sublayers)."""
+    import copy
+
+    import unet_block as UB
+    lv = UB.LEVELS[level]
+    blk = UB.build(lv, gpu)
+    fused = UB.to_fused16(copy.deepcopy(blk))
+    x, ctx = UB.inputs(lv, gpu)
+    dy = torch.randn_like(x)
+    got = []
+    for b in (blk, fused):
+        t = x.detach().requires_grad_(True)
+        y = b(t, ctx)
+        got.append((y.detach(), *torch.autograd.grad(y, [t, *b.parameters()], dy)))
+    names = ["y", "dx"] + [n for n, _ in blk.named_parameters()]
+    for n, a, b in zip(names, *got):
+        rel = float((a.double() - b.double()).norm() / a.double().norm())
+        assert rel < 16 * 2.0 ** -11, (n, rel)
+    with torch.no_grad():
+        assert torch.equal(fused(x, ctx), got[1][0])

@@ -11,7 +11,9 @@ stamps the INT8 backend on the cross-attention as well, and
 ``quantize_linears`` swaps any of the block's linears for W8A8 layers. With
 W8A8 ``proj`` and ``out`` layers the feed-forward runs the fused GEGLU middle
 (``int8_geglu_ff``), where the reference would run ``x * F.gelu(gate)`` on the
-dequantized activations.
+dequantized activations. A block that stays in 16 bits, for inference or
+training, can run its norms and feed-forward on the package's trainable kernels
+instead of torch's ops (:func:`to_fused16`).
 
 This is a measurement and test harness (``bench.py --shapes``,
 ``tests/test_gpu_unet.py``), not a product model.
@@ -25,7 +27,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from diffucore_amd import attention_bhld
+from diffucore_amd import attention_bhld, geglu_ff, layer_norm
 from diffucore_amd._int8 import Int8Linear, int8_geglu_ff
 
 
@@ -113,8 +115,15 @@ class BasicTransformerBlock(nn.Module):
         self.ff = FeedForward(dim)
         self.attn2 = CrossAttention(dim, context_dim, heads, dim_head)
         self.norm1, self.norm2, self.norm3 = nn.LayerNorm(dim), nn.LayerNorm(dim), nn.LayerNorm(dim)
+        self.fused16 = False   # see to_fused16
 
     def forward(self, x: torch.Tensor, context: torch.Tensor) -> torch.Tensor:
+        if self.fused16:
+            def norm(m, x):
+                return layer_norm(x, m.weight, m.bias, m.eps)
+            x = x + self.attn1(norm(self.norm1, x))
+            x = x + self.attn2(norm(self.norm2, x), context)
+            return geglu_ff(norm(self.norm3, x), self.ff.net[0].proj, self.ff.net[2], residual=x)
         x = x + self.attn1(self.norm1(x))
         x = x + self.attn2(self.norm2(x), context)
         return x + self.ff(self.norm3(x))
@@ -161,6 +170,14 @@ def to_int8(blk: BasicTransformerBlock, device) -> BasicTransformerBlock:
     blk.attn1.qkv_fused = fuse_linears([blk.attn1.to_q, blk.attn1.to_k, blk.attn1.to_v])
     blk.attn2.kv_fused = fuse_linears([blk.attn2.to_k, blk.attn2.to_v])
     set_attention_backend(blk, "int8_turing")
+    return blk
+
+
+def to_fused16(blk: BasicTransformerBlock) -> BasicTransformerBlock:
+    """Run the block's three norms and its feed-forward, with the residual, on
+    ``layer_norm`` and ``geglu_ff`` (16-bit layers, trainable); the attentions
+    stay as they are."""
+    blk.fused16 = True
     return blk
 
 
