@@ -132,19 +132,23 @@ int reduce_partials(const float* part, int P, int sections, int64_t width, void*
   return launch_status(what);
 }
 
-// The split of an [M, N] pass: TX lanes of 8 columns (a power of two, at most
-// 64), and row blocks so that about 8 workgroups per CU run, each with at
-// least 4 rows a lane.
+// The split of an [M, N] pass: TX lanes of 8 columns, the most (a power of two,
+// 64 at most) that leave no more than an eighth of them idle past the row's end,
+// but 16 where rows have as many; and row blocks so that about 8 workgroups per
+// CU run, down to one row a lane. 777 x 2731 gated bf16 18.6 -> 11.9 us, 1001 x
+// 577 fp16 10.8 -> 5.4 against 4 rows a lane on 64 lanes.
 struct ActBwdPlan {
   int tx_log, rows, col_blocks, row_blocks;
 };
 static ActBwdPlan act_bwd_plan(int64_t M, int64_t N) {
   ActBwdPlan r;
-  r.tx_log = 0;
-  while (r.tx_log < 6 && (8LL << r.tx_log) < N) ++r.tx_log;
-  const int64_t pad = (N + 63) / 64 * 64, TY = 256 >> r.tx_log;   // the columns of dz
-  r.col_blocks = (int)((pad + (8LL << r.tx_log) - 1) / (8LL << r.tx_log));
-  const int64_t most = (M + 4 * TY - 1) / (4 * TY);
+  const int64_t chunks = dz_width(N) / 8;   // of a row of dz
+  for (r.tx_log = 6; r.tx_log > 3; --r.tx_log) {
+    const int64_t TX = 1LL << r.tx_log, idle = (chunks + TX - 1) / TX * TX - chunks;
+    if (8 * idle <= chunks || (r.tx_log == 4 && chunks >= 16)) break;
+  }
+  const int64_t TX = 1LL << r.tx_log, TY = 256 >> r.tx_log, most = (M + TY - 1) / TY;
+  r.col_blocks = (int)((chunks + TX - 1) / TX);
   int64_t want = (8LL * device_cus() + r.col_blocks - 1) / r.col_blocks;
   if (want > most) want = most;
   if (want < 1) want = 1;

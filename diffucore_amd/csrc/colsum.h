@@ -12,9 +12,13 @@ int reduce_partials(const float* part, int P, int sections, int64_t width, void*
                     hipStream_t st, const char* what);
 
 // The elementwise half of a feed-forward backward pass: dz of dy and the
-// pre-activations (zg: gated; neither: none), rows of lddz = N rounded up to 64
-// with zeros past N, and the sums of dz over rows before rounding (NULL: not
+// pre-activations (zg: gated; neither: none), rows of lddz = dz_width(N) with
+// zeros past N, and the sums of dz over rows before rounding (NULL: not
 // asked for). `part`: act16_bwd_part_bytes of scratch for the sums.
+// A dz row: whole stages of 64, with 8 zeros past N rounded up to 8 unless N is
+// a multiple of 64.
+inline int64_t dz_width(int64_t N) { return (N + 63) / 64 * 64 + (N % 64 > 56 ? 64 : 0); }
+
 struct ActBwd {
   const void* dy;
   int64_t lddy;

@@ -175,6 +175,13 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
                : "memory");
 }
 
+// The same from an address of each lane's own.
+__device__ __forceinline__ void dma16_at(const void* lane, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
 // vmcnt(n) with the other counters left unconstrained, and lgkmcnt(0) (gfx9
 // encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
 template <int N>

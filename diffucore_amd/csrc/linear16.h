@@ -23,7 +23,8 @@
 //   block fall on different banks, and so do the two blocks of a 32-row fragment.
 //
 // The contraction's end inside a stage: loads clamp to the last k (rows to the
-// last row), and the last stage's fragments are masked.
+// last row), and the last stage's fragments are masked. Of two terms the first
+// ends on whole stages: A has zeros up to there, and w's lines are read as zeros.
 #pragma once
 
 #include "colsum.h"
@@ -38,6 +39,7 @@ struct Gemm16 {
   int K;                    // k of a term
   int ka;                   // k that a term's A rows (KC) can be read to, a multiple of 8
   int nk1, nk;              // stages of the first term, and of all
+  const uint16_t* zeros;    // two terms: 16 bytes of zeros, 16-byte aligned
   int wlim, alim;           // rows of W and A that loads may touch (RC: rounded up to 8)
   int tiles_m, tiles_n;
   int problems;             // 2: a second product (a2, out2) in the same launch
@@ -321,7 +323,15 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
         const int r = 8 * (w + T::NW * u) + lane / 8, c = (lane % 8) ^ ((r >> 1) & 7), ln = rc_line(u, BN);
         const uint32_t o = W_RC ? woff[u] - (uint32_t)(ln - min(ln, left - 1)) * (uint32_t)p.ldw * 2
                                 : woff[u] - 16 * (c - min(c, last));
-        dma16(GATED && (((w + T::NW * u) / 4) & 1) ? gb : wb, o, d + 1024 * T::NW * u);
+        if constexpr (W_RC && !A_RC) {
+          // where a first term ends, its A holds zeros that meet w's lines past the
+          // end: zeros too, as 0 times an infinite w would be NaN
+          const uint8_t* at = reinterpret_cast<const uint8_t*>(wb) + o;
+          if (p.zeros && ln >= left) at = reinterpret_cast<const uint8_t*>(p.zeros);
+          dma16_at(at, d + 1024 * T::NW * u);
+        } else {
+          dma16(GATED && (((w + T::NW * u) / 4) & 1) ? gb : wb, o, d + 1024 * T::NW * u);
+        }
       }
 #pragma unroll
       for (int u = 0; u < T::LA; ++u) {
@@ -420,21 +430,15 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
   sync();
   int slot = 0;
   if (kt + 1 < kend) frags(0, 0, 0);
-  // The first of two terms may end inside a stage too: the zeros that A holds
-  // there do not do, as 0 times an infinite w is NaN.
-  constexpr bool TERMS = W_RC && !A_RC;
-  const int mask_at = TERMS && p.nk > p.nk1 && p.K % 64 ? p.nk1 - 1 : -1;
   // stage kt in `slot`; MORE: stage kt + S exists
   auto stage = [&](auto more) __attribute__((always_inline)) {
     constexpr bool MORE = decltype(more)::value;
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks) {
-      if (TERMS && kt == mask_at) mask(ks & 1, ks, p.K % 64);
       frags((ks + 1) & 1, slot, ks + 1);
       mfmas(ks & 1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (TERMS && kt == mask_at) mask(1, 3, p.K % 64);
     const int next = slot == S - 1 ? 0 : slot + 1;
     if constexpr (MORE) wait_vmcnt<(S - 2) * L>();
     else wait_left(kend - 2 - kt);

@@ -18,12 +18,12 @@ struct Backward16 {
   Backward16(const Mat16& dy_, const Mat16& x_, const Mat16& wv_, const Mat16& wg_, bool z_, bool want_dx, int want_dw,
              bool want_db, void* base)
       : dy(dy_), x(x_), wv(wv_), wg(wg_), z(z_) {
-    const int64_t M = dy.rows, N = dy.width, K = x.width, N64 = round_up(N, 64);
+    const int64_t M = dy.rows, N = dy.width, K = x.width, ldz = dz_width(N);
     const bool gated = wg.p;
     Scratch16 s{static_cast<uint8_t*>(base)};
     if (z) {
-      dz = {s.take(2 * (size_t)M * N64), N64, M, N64};
-      if (gated) dzg = {s.take(2 * (size_t)M * N64), N64, M, N64};
+      dz = {s.take(2 * (size_t)M * ldz), ldz, M, ldz};
+      if (gated) dzg = {s.take(2 * (size_t)M * ldz), ldz, M, ldz};
       else dzg = {};
     } else {
       dz = want_dx || want_dw ? s.operand(dy) : dy;
@@ -33,7 +33,7 @@ struct Backward16 {
     wvs = want_dx ? s.operand(wv) : wv;
     wgs = want_dx && gated ? s.operand(wg) : wg;
     // the passes run one after the other: their partial sums share one place
-    const int64_t nk = N64 / 64;
+    const int64_t nk = round_up(N, 64) / 64;
     problems = want_dw == 2 ? 2 : 1;
     dx_plan = plan16(M, K, gated ? 2 * nk : nk, 1);
     dw_plan = plan16(N, K, round_up(M, 64) / 64, problems);
@@ -62,6 +62,7 @@ static int run_dx(const char* who, const Backward16& b, void* dx, int64_t lddx, 
   p.M = (int)M, p.N = (int)K, p.K = (int)N, p.ka = (int)b.dz.width;
   p.nk1 = (int)(N64 / 64), p.nk = b.wg.p ? 2 * p.nk1 : p.nk1;
   p.alim = (int)M, p.wlim = (int)round_up(K, 8);
+  if (b.wg.p && N % 64) p.zeros = p.a + round_up(N, 8);   // of dz's first row
   p.out = static_cast<uint16_t*>(dx), p.ldo = lddx;
   p.problems = 1, p.part = b.part, p.width = (int)K;
   return dtype == DC_BF16 ? run_tile16<DC_BF16, false, true, EPI_NONE>(who, p, b.dx_plan, st)
@@ -132,7 +133,7 @@ extern "C" int dc_linear16_bwd(const void* dy, int64_t lddy, const void* x, int6
   if (int e = b.pad(who, st)) return e;
   if (act_z || db) {
     const ActBwd a{dy, lddy, static_cast<const uint8_t*>(act_z ? z : nullptr), nullptr, act,
-                   const_cast<void*>(act_z ? b.dz.p : nullptr), nullptr, round_up(N, 64), db, nullptr, db_dtype, dtype,
+                   const_cast<void*>(act_z ? b.dz.p : nullptr), nullptr, dz_width(N), db, nullptr, db_dtype, dtype,
                    M, N, b.part};
     if (int e = act16_bwd(who, a, st)) return e;
   }
