@@ -58,22 +58,6 @@ inline int device_cus() {
   return n;
 }
 
-// Sets a kernel's dynamic LDS limit, once per instantiation and device
-// (`done`: its flags); threads that race on a first call each set it (the call
-// is idempotent).
-inline int reserve_lds(const void* fn, int bytes, std::atomic<bool> (&done)[64], const char* what) {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (done[dev].load(std::memory_order_acquire)) return DC_OK;
-  hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != hipSuccess) {
-    set_error("%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
-    return DC_EHIP;
-  }
-  done[dev].store(true, std::memory_order_release);
-  return DC_OK;
-}
-
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 inline int elem_bytes(int dtype) {
@@ -174,22 +158,6 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
                "{m0}"(__builtin_amdgcn_readfirstlane(lds))
                : "memory");
 }
-
-// The same from an address of each lane's own.
-__device__ __forceinline__ void dma16_at(const void* lane, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane),
-               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory");
-}
-
-// vmcnt(n) with the other counters left unconstrained, and lgkmcnt(0) (gfx9
-// encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-  static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
-__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4)); }
 
 // ---------------------------------------------------------------- wave reductions
 

@@ -698,6 +698,15 @@ typedef DmaTile<2, 4, 1, 1, 3, 128, 4> Dma64x128;     // 8 waves of 32 x 32, 72 
 typedef DmaTile<2, 2, 1, 1, 3, 128, 3> Dma64x64;      // 4 waves of 32 x 32, 48 KB: 3 per CU
 typedef DmaTile<2, 2, 2, 2, 3, 64, 3> Dma128x128k;    // 4 waves of 64 x 64, 48 KB, 64-byte stages: 3 per CU
 
+// vmcnt(n) with the other counters left unconstrained, and lgkmcnt(0) (gfx9
+// encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4)); }
+
 // RES: with the gated residual of dc_w8a8_gemm_grouped_gated.
 template <class T, int OUT_DT, int BIAS_DT, bool RES = false>
 __global__ void __launch_bounds__(T::NT, T::OCC) w8a8_gemm_dma_kernel(GemmArgs p, GroupArgs g) {
@@ -910,6 +919,22 @@ __global__ void __launch_bounds__(256) rescale_vec_kernel(const int32_t* __restr
     const uint32_t hi = f32_to_h16<OUT_DT>(y2) | (f32_to_h16<OUT_DT>(y3) << 16);
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + m * ldo + n) = make_uint2(lo, hi);
   }
+}
+
+// Sets a kernel's dynamic LDS limit, once per instantiation and device
+// (`done`: its flags); threads that race on a first call each set it (the call
+// is idempotent).
+static int reserve_lds(const void* fn, int bytes, std::atomic<bool> (&done)[64], const char* what) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (done[dev].load(std::memory_order_acquire)) return DC_OK;
+  hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    set_error("%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    return DC_EHIP;
+  }
+  done[dev].store(true, std::memory_order_release);
+  return DC_OK;
 }
 
 template <class T, int OUT_DT, int BIAS_DT>

@@ -31,6 +31,38 @@
 
 namespace dc {
 
+// One DMA of 16 bytes per lane into LDS (see dma16) from an address of each lane's own.
+__device__ __forceinline__ void dma16_at(const void* lane, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane),
+               "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
+// As in gemm.hip: vmcnt(n) with the other counters left unconstrained, and lgkmcnt(0) (gfx9
+// encoding: vmcnt bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+__device__ __forceinline__ void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4)); }
+
+// Sets a kernel's dynamic LDS limit, once per instantiation and device
+// (`done`: its flags); threads that race on a first call each set it (the call
+// is idempotent).
+inline int reserve_lds(const void* fn, int bytes, std::atomic<bool> (&done)[64], const char* what) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (done[dev].load(std::memory_order_acquire)) return DC_OK;
+  hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    set_error("%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+    return DC_EHIP;
+  }
+  done[dev].store(true, std::memory_order_release);
+  return DC_OK;
+}
+
 struct Gemm16 {
   const uint16_t *a, *a2;   // a2: the second term's (terms == 2) or second problem's A
   const uint16_t *w, *w2;   // w2: the second term's W, or the gate's
