@@ -50,10 +50,9 @@ def _act(z: torch.Tensor, act: str) -> torch.Tensor:
 
 # ─── argument checks ─────────────────────────────────────────────────────────
 
-def _check_act(what: str, act: str, gated: bool = False) -> int:
-    if act not in ACTIVATIONS or (gated and act == "none"):
-        allowed = sorted(a for a in ACTIVATIONS if not (gated and a == "none"))
-        raise ValueError(f"{what}: act must be one of {allowed}, got {act!r}")
+def _check_act(what: str, act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{what}: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
     return ACTIVATIONS[act]
 
 
@@ -83,6 +82,8 @@ def _check_product(what: str, x: torch.Tensor, weight: torch.Tensor) -> None:
     if x.is_cuda:
         if x.dtype not in _HALF:
             raise TypeError(f"{what}: the kernels take fp16 or bf16 tensors, got {x.dtype}")
+    elif x.dtype not in _FLOAT:
+        raise TypeError(f"{what}: x is {x.dtype}, expected fp16, bf16 or float32")
     elif not _host(x):
         raise RuntimeError(f"{what}: diffucore_amd runs on GPU and CPU tensors (got a {x.device} tensor)")
 
@@ -326,9 +327,9 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     holds the value rows and then the gate rows (the GEGLU projection's layout,
     as :func:`geglu_quantize` takes it), or, with ``gate_weight [F, K]``, the
     value rows alone (``weight [F, K]``); the biases likewise. ``act`` is one of
-    :data:`ACTIVATIONS` except ``"none"``. Types as in :func:`linear_act`."""
+    :data:`ACTIVATIONS` (``"none"``: the plain product). Types as in :func:`linear_act`."""
     what = "gated_linear"
-    code = _check_act(what, act, gated=True)
+    code = _check_act(what, act)
     _check_product(what, x, weight)
     N = weight.shape[0]
     if gate_weight is not None:

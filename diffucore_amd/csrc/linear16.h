@@ -108,7 +108,8 @@ struct Tile16 {
 template <int DT>
 __device__ __forceinline__ v16f mfma16(v4i w, v4i a, v16f c) {
   if constexpr (DT == DC_BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, a), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, a), c, 0, 0,
+                                                   0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, a), c, 0, 0, 0);
 }
@@ -536,8 +537,7 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
     // one uniform branch around the whole of it, so that the steps of a block overlap
     with_act(p.act, [&](auto act_) __attribute__((always_inline)) {
       constexpr int ACT = decltype(act_)::value;
-      if constexpr (GATED && ACT == DC_ACT_NONE) return;   // refused by the host
-      rows_pre<FN, FM, GATED>(acc, share, lane, [&](int r, float (&v)[8], float (&g)[8]) __attribute__((always_inline)) {
+      auto put = [&](int r, float (&v)[8], float (&g)[8]) __attribute__((always_inline)) {
         const int m = mb + r;
         if (m >= p.M || n >= p.N) return;
 #pragma unroll
@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(T::NT, T::OCC) linear16_kernel(Gemm16 p) {
           for (int e = 0; e < 8; ++e) v[e] += s[e];
         }
         store_chunk16(p.out + (int64_t)m * p.ldo + n, p.N - n, pack8<DT>(v));
-      });
+      };
+      rows_pre<FN, FM, GATED>(acc, share, lane, put);
     });
   } else {
     rows_h16<DT, FN, FM>(acc, share, lane, [&](int r, int c, uint4 v) __attribute__((always_inline)) {

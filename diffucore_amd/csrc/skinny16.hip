@@ -20,7 +20,8 @@ constexpr int SKINNY_WAVES = 8, SKINNY_CH = 16;
 template <int DT>
 __device__ __forceinline__ v4f mfma16x16(uint4 w, uint4 x, v4f c) {
   if constexpr (DT == DC_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0,
+                                                   0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), c, 0, 0, 0);
 }

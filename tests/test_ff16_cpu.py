@@ -42,7 +42,7 @@ def test_linear_act_on_cpu_tensors(act, dt):
         _within(g.reshape(value.shape), value, bound + O.U[dt] * value.abs() * 4 + 1e-6, name)
 
 
-@pytest.mark.parametrize("act", [a for a in ACTS if a != "none"])
+@pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("fused", [True, False])
 def test_gated_linear_on_cpu_tensors(act, fused):
     x, wv, wg = _rand(5, 12), _rand(6, 12, seed=1), _rand(6, 12, seed=2)
@@ -81,8 +81,6 @@ def test_oracle_gradients_against_differences(act):
                        ("db", b, lambda t: (O.linear(x, w, t, act, None, dt)["y"][0] * dy).sum())):
         v = _rand(*t.shape, seed=9, dtype=torch.float64)
         assert abs(float((got[name][0] * v).sum()) - _difference(f, t, v)) < 1e-6, name
-    if act == "none":
-        return
     got = O.gated(x, w, wg, b, bg, act, dt, dy)
     for name, i in (("dx", 0), ("dw", 1), ("dwg", 2), ("db", 3), ("dbg", 4)):
         args = [x, w, wg, b, bg]
@@ -123,7 +121,10 @@ def test_empty_inputs():
 
 @pytest.mark.parametrize("call, error, match", [
     (lambda x, w, b: D.linear_act(x, w, b, act="relu6"), ValueError, "act must be one of"),
-    (lambda x, w, b: D.gated_linear(x, w, b, act="none"), ValueError, "act must be one of"),
+    (lambda x, w, b: D.gated_linear(x, w, b, act="geglu"), ValueError, "act must be one of"),
+    (lambda x, w, b: D.linear_act(x.double(), w.double()), TypeError, "x is"),
+    (lambda x, w, b: D.gated_linear(x.double(), w.double()), TypeError, "x is"),
+    (lambda x, w, b: D.linear_act(x.int(), w.int()), TypeError, "x is"),
     (lambda x, w, b: D.linear_act(x, w.t(), b), ValueError, "weight is"),
     (lambda x, w, b: D.linear_act(x, w[0], b), ValueError, "1-dimensional"),
     (lambda x, w, b: D.linear_act(x, w, b[:3]), ValueError, "bias is"),

@@ -141,6 +141,13 @@ def test_linear_large(gpu, M, K, N, dt):
     _check_linear(M, K, N, dt, "gelu_tanh", res=True)
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M", [3, 130])
+def test_gated_activations(gpu, act, M):
+    _check_gated(M, 96, 136, DTYPES[M % 2], act)
+    _check_gated(M, 1024, 136, DTYPES[1 - M % 2], act, bias=False, fused=False)
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("fused", [True, False])
 @pytest.mark.parametrize("M", [1, 5, 16, 17, 40, 128, 333, 1100])
@@ -152,7 +159,7 @@ def test_gated_rows(gpu, M, fused, dt):
                                   (1000, 2731), (2560, 640), (24, 2000)])
 @pytest.mark.parametrize("M", [1, 19, 260])
 def test_gated_widths(gpu, M, K, N):
-    act = [a for a in ACTS if a != "none"][(K + N) % 4]
+    act = ACTS[(K + N) % len(ACTS)]
     _check_gated(M, K, N, DTYPES[(M + K) % 2], act, bias=(K + M) % 3 != 0, fused=(K + N + M) % 2 == 0, seed=K + N)
 
 
