@@ -401,7 +401,7 @@ int dc_int8_attn_quantize_q(const void* q, int dtype, int B, int H, int Lq, int 
  * NULL) of bias_dtype, which is `dtype` or DC_F32, res [M, N] or NULL, act DC_ACT_NONE / GELU_ERF /
  * GELU_TANH / SILU / QUICK_GELU. z (or NULL; 2-byte aligned,
  * dc_saved16_bytes) takes the pre-activation x w^T + bias for dc_linear16_bwd:
- * the upper 24 bits of its float32 values, a plane of halves and one of bytes.
+ * its float32 values to 16 significant bits, a plane of halves and one of bytes.
  */
 size_t dc_saved16_bytes(int64_t M, int64_t N);
 size_t dc_linear16_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N,

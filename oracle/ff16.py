@@ -6,7 +6,7 @@ most ``u |y|`` (``u`` half a step of its type, plus half the smallest
 subnormal) and by the float32 sum's error, ``(n + 16) 2^-23`` times the sum of
 the terms' magnitudes for ``n`` terms (twice the textbook ``n 2^-24``: matrix
 cores add in groups, and an activation adds a few ulp of its own). The backward
-passes of an activation start from its input cut to 24 bits (``2^-16`` of it):
+passes of an activation start from its input kept to ``2^-16`` of itself:
 that and the sum's error move a slope by at most ``max|act''|`` (below 1.2 for
 every activation here) times themselves and a value by ``max|act'|`` (below
 1.2), and the products' operand ``dz`` is rounded to 16 bits once.

@@ -346,6 +346,36 @@ def test_gpu_refusals(gpu):
         D.layer_norm(x, bias=torch.zeros(8))
 
 
+# ---------------------------------------------------------------- random shapes
+
+def random_call(seed):
+    """One call of random sizes (over their logarithm, every third one a
+    multiple of 64), types, layout and strides, checked in full."""
+    import random
+    rng = random.Random(seed)
+    size = lambda lo, hi: int(2.0 ** rng.uniform(lo, hi))   # noqa: E731
+    wide = lambda lo, hi: size(lo, hi) if rng.random() < 2 / 3 else -(-size(lo, hi) // 64) * 64   # noqa: E731
+    dt = rng.choice(DTYPES)
+    kind = rng.choice(["linear", "gated", "norm"])
+    M = size(0, 11.5)
+    if kind == "norm":
+        dt = rng.choice([*DTYPES, torch.float32])
+        return _check_norm(M, wide(0, 14), dt, rng.choice([None, torch.float32]), seed=seed)
+    K, N = wide(0, 11.5), wide(0, 11.5)
+    g = _gen(seed)
+    pad = rng.choice([0, 0, 8, 3])
+    x = _rand(g, M, K + pad, dtype=dt)[:, :K]
+    bias_dt = rng.choice([None, torch.float32])
+    if kind == "linear":
+        return _check_linear(M, K, N, dt, rng.choice(ACTS), rng.random() < 0.7, rng.random() < 0.5, seed, bias_dt, x=x)
+    return _check_gated(M, K, N, dt, rng.choice(ACTS), rng.random() < 0.7, rng.random() < 0.5, seed, bias_dt, x=x)
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_random_calls(gpu, seed):
+    random_call(seed)
+
+
 # ---------------------------------------------------------------- past 32 bits
 
 def test_layer_norm_past_32_bits(gpu):
